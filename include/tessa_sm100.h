@@ -670,6 +670,75 @@ TESSA_API int tessa_replay_session_create(int device, const tessa_prepared_repla
 TESSA_API int tessa_replay_run_mode(tessa_replay_session* session, uint32_t mode, tessa_mode_result* result);
 TESSA_API void tessa_replay_session_destroy(tessa_replay_session* session);
 
+/* ------------------------------------------- training the vectors --- */
+
+/* Operators that train a table of vectors on neighbour lists: rows out of the
+ * table and their gradient, an FP8 product with a scale per block of 128, and
+ * the distillation loss from a teacher's top-k list.  They have no counterpart
+ * in the reference.
+ *
+ * These calls only enqueue work on `stream` and return: nothing waits for the
+ * device, no scratch is kept in the context (where one is needed the caller
+ * passes `workspace`, 256-byte aligned, of the size that the matching
+ * *_workspace function gives; it is free again when the call's work is done),
+ * and they may be captured into a CUDA graph.  What a kernel finds wrong (an
+ * id outside the table: TESSA_ERR_BAD_ROW; an expired wait: TESSA_ERR_TIMEOUT)
+ * is therefore reported by the next of these calls on the context, or by
+ * tessa_async_status, which waits for `stream` first; either report clears it.
+ * A bad id is never read through: its row counts as padding.
+ *
+ * Matrices are row-major device memory with `stride` elements from row to row
+ * (stride >= columns); element types: */
+#define TESSA_F32 0
+#define TESSA_BF16 1
+#define TESSA_F16 2
+
+TESSA_API int tessa_async_status(tessa_ctx* ctx, void* stream);
+
+/* out[t] = scale * table[ids[t]], computed in f32 and rounded once to out's
+ * type.  ids: signed 32- or 64-bit (id_bits); -1 is padding and gives a row of
+ * zeros. */
+typedef struct tessa_lookup_args {
+  const void* table;
+  uint64_t table_rows;          /* below 2^32 - 1 */
+  uint64_t table_stride;
+  uint32_t dim;
+  uint32_t dtype;
+  const void* ids;
+  uint32_t id_bits;             /* 32 or 64 */
+  uint32_t out_dtype;
+  uint64_t count;               /* ids, below 2^31 */
+  float scale;
+  void* out;                    /* count x dim */
+  uint64_t out_stride;
+} tessa_lookup_args;
+TESSA_API int tessa_embedding_lookup(tessa_ctx* ctx, const tessa_lookup_args* args, void* stream);
+
+/* Gradient of tessa_embedding_lookup: grad[v] = scale * sum of dout[t] over
+ * the t with ids[t] == v, for every row v of the table (rows that no id names
+ * become zero), or, with accumulate, grad[v] += that sum (rows that no id
+ * names are not touched).  The ids are sorted by (id, t), and each row's sum
+ * runs over its t in that order in f32 with one rounding at the end: the same
+ * inputs give the same bits. */
+typedef struct tessa_lookup_grad_args {
+  const void* dout;             /* count x dim */
+  uint64_t dout_stride;
+  uint32_t dim;
+  uint32_t dtype;
+  const void* ids;
+  uint32_t id_bits;
+  uint32_t grad_dtype;
+  uint64_t count;
+  float scale;
+  uint32_t accumulate;          /* 0 or 1 */
+  void* grad;                   /* table_rows x dim */
+  uint64_t grad_stride;
+  uint64_t table_rows;
+} tessa_lookup_grad_args;
+TESSA_API int tessa_embedding_grad_workspace(uint64_t count, uint64_t table_rows, uint32_t dim, uint64_t* bytes);
+TESSA_API int tessa_embedding_grad(tessa_ctx* ctx, const tessa_lookup_grad_args* args, void* workspace,
+                                   uint64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

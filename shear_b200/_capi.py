@@ -149,6 +149,24 @@ class CompactView(ctypes.Structure):
     ]
 
 
+class LookupArgs(ctypes.Structure):
+    _fields_ = [
+        ("table", c_vp), ("table_rows", ctypes.c_uint64), ("table_stride", ctypes.c_uint64),
+        ("dim", ctypes.c_uint32), ("dtype", ctypes.c_uint32), ("ids", c_vp), ("id_bits", ctypes.c_uint32),
+        ("out_dtype", ctypes.c_uint32), ("count", ctypes.c_uint64), ("scale", ctypes.c_float), ("out", c_vp),
+        ("out_stride", ctypes.c_uint64),
+    ]
+
+
+class LookupGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("dout", c_vp), ("dout_stride", ctypes.c_uint64), ("dim", ctypes.c_uint32), ("dtype", ctypes.c_uint32),
+        ("ids", c_vp), ("id_bits", ctypes.c_uint32), ("grad_dtype", ctypes.c_uint32), ("count", ctypes.c_uint64),
+        ("scale", ctypes.c_float), ("accumulate", ctypes.c_uint32), ("grad", c_vp),
+        ("grad_stride", ctypes.c_uint64), ("table_rows", ctypes.c_uint64),
+    ]
+
+
 # (name, restype, argtypes) for every entry point of include/tessa_sm100.h
 SIGNATURES = [
     ("tessa_abi_version", ctypes.c_int, []),
@@ -212,6 +230,11 @@ SIGNATURES = [
     ("tessa_reduce_grouped", ctypes.c_int,
      [c_vp, ctypes.c_uint32, c_vp, c_vp, c_vp, ctypes.c_uint64, ctypes.c_uint32, c_vp, c_vp, c_vp,
       ctypes.c_uint64, ctypes.POINTER(ctypes.c_uint64), c_vp]),
+    ("tessa_async_status", ctypes.c_int, [c_vp, c_vp]),
+    ("tessa_embedding_lookup", ctypes.c_int, [c_vp, ctypes.POINTER(LookupArgs), c_vp]),
+    ("tessa_embedding_grad_workspace", ctypes.c_int,
+     [ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint32, ctypes.POINTER(ctypes.c_uint64)]),
+    ("tessa_embedding_grad", ctypes.c_int, [c_vp, ctypes.POINTER(LookupGradArgs), c_vp, ctypes.c_uint64, c_vp]),
 ]
 
 _lib = None

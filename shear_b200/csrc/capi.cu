@@ -284,6 +284,7 @@ struct tessa_ctx {
   DevBuf probe;                     // bounded-wait probe: elapsed time
   SubmitRing* ring = nullptr;       // subtree submissions (created on first use)
   uint32_t leaf_kernel = 1;         // 0: column-split kernel on CTA pairs where it applies, 1: one CTA per tile
+  uint32_t* async_err = nullptr;    // pinned, mapped error word of the calls that do not wait (created on first use)
 };
 
 namespace {
@@ -303,6 +304,16 @@ int read_err(tessa_ctx* ctx, cudaStream_t st, uint32_t* bits) {
 int clear_err(tessa_ctx* ctx, cudaStream_t st) {
   CUDA_TRY(cudaMemsetAsync(ctx->d_err.ptr, 0, 4, st));
   return TESSA_OK;
+}
+
+// Error bits that kernels of the calls that do not wait have left so far;
+// taking them clears the word.
+int take_async_error(tessa_ctx* ctx) {
+  if (!ctx->async_err) return TESSA_OK;
+  const uint32_t bits = *reinterpret_cast<volatile uint32_t*>(ctx->async_err);
+  if (bits == 0) return TESSA_OK;
+  *reinterpret_cast<volatile uint32_t*>(ctx->async_err) = 0;
+  return map_device_error(bits);
 }
 
 // Blocked scans: the inner loops have no early exit, so they vectorise.
@@ -752,7 +763,30 @@ int assign_device(tessa_ctx* ctx, uint32_t source, const tessa_assign_args* a, c
 
 }  // namespace
 
+int tessa::async_begin(tessa_ctx* ctx, AsyncCtx* out) {
+  TRY(bind(ctx));
+  if (!ctx->async_err) {
+    void* p = nullptr;
+    CUDA_TRY(cudaHostAlloc(&p, 64, cudaHostAllocMapped));
+    memset(p, 0, 64);
+    ctx->async_err = static_cast<uint32_t*>(p);
+  }
+  TRY(take_async_error(ctx));
+  out->sm_count = ctx->sm_count;
+  out->timeout_ns = ctx->timeout_ns;
+  void* d = nullptr;
+  CUDA_TRY(cudaHostGetDevicePointer(&d, ctx->async_err, 0));
+  out->err = static_cast<uint32_t*>(d);
+  return TESSA_OK;
+}
+
 extern "C" {
+
+int tessa_async_status(tessa_ctx* ctx, void* stream) {
+  TRY(bind(ctx));
+  CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
+  return take_async_error(ctx);
+}
 
 int tessa_abi_version(void) { return TESSA_ABI_VERSION; }
 
@@ -831,6 +865,10 @@ void tessa_destroy(tessa_ctx* ctx) {
       cudaStreamSynchronize(s);
       cudaStreamDestroy(s);
     }
+  if (ctx->async_err) {
+    cudaDeviceSynchronize();  // kernels in flight may still write the word
+    cudaFreeHost(ctx->async_err);
+  }
   for (cudaEvent_t e : ctx->d0_ev)
     if (e) cudaEventDestroy(e);
   for (cudaEvent_t e : ctx->ev_in) cudaEventDestroy(e);

@@ -1,0 +1,115 @@
+// C ABI of the operators that train a table of vectors (lookup, FP8 product,
+// distillation): argument checks before any launch.  These calls enqueue and
+// return; see the header on how device-side errors are reported.
+#include <cstdarg>
+#include <cstdio>
+
+#include "kernels.h"
+
+using namespace tessa;
+
+namespace {
+
+int bad(int code, const char* fmt, ...) {
+  char buf[256];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return set_last_error(code, buf);
+}
+
+#define TRY(expr)                \
+  do {                           \
+    int _r = (expr);             \
+    if (_r != TESSA_OK) return _r; \
+  } while (0)
+
+typedef unsigned long long ull;
+
+uint32_t elem_bytes(uint32_t dtype) { return dtype == TESSA_F32 ? 4u : 2u; }
+
+int check_dtype(const char* what, uint32_t dtype) {
+  if (dtype > TESSA_F16) return bad(TESSA_ERR_INVALID_ARG, "%s: unknown element type %u", what, dtype);
+  return TESSA_OK;
+}
+
+// A matrix argument: pointer present and element-aligned, stride of at least a row.
+int check_matrix(const char* what, const void* p, uint64_t rows, uint64_t cols, uint64_t stride, uint32_t dtype) {
+  TRY(check_dtype(what, dtype));
+  if (rows == 0 || cols == 0) return TESSA_OK;
+  if (!p) return bad(TESSA_ERR_INVALID_ARG, "%s: null pointer", what);
+  if (reinterpret_cast<uintptr_t>(p) % elem_bytes(dtype))
+    return bad(TESSA_ERR_INVALID_ARG, "%s: not aligned to its element type", what);
+  if (rows > 1 && stride < cols)
+    return bad(TESSA_ERR_INVALID_ARG, "%s: stride %llu below %llu columns", what, (ull)stride, (ull)cols);
+  if (stride > (1ull << 40)) return bad(TESSA_ERR_UNSUPPORTED, "%s: stride %llu above 2^40", what, (ull)stride);
+  return TESSA_OK;
+}
+
+int check_ids(const void* ids, uint32_t id_bits, uint64_t count) {
+  if (id_bits != 32 && id_bits != 64) return bad(TESSA_ERR_INVALID_ARG, "ids of %u bits: 32 or 64", id_bits);
+  if (count && !ids) return bad(TESSA_ERR_INVALID_ARG, "ids: null pointer");
+  if (reinterpret_cast<uintptr_t>(ids) % (id_bits / 8))
+    return bad(TESSA_ERR_INVALID_ARG, "ids: not aligned to their type");
+  return TESSA_OK;
+}
+
+int check_workspace(const void* ws, uint64_t have, uint64_t need) {
+  if (need == 0) return TESSA_OK;
+  if (!ws || have < need)
+    return bad(TESSA_ERR_INVALID_ARG, "workspace of %llu bytes, %llu needed", (ull)(ws ? have : 0), (ull)need);
+  if (reinterpret_cast<uintptr_t>(ws) % 256) return bad(TESSA_ERR_INVALID_ARG, "workspace not 256-byte aligned");
+  return TESSA_OK;
+}
+
+int launched(const char* what, cudaError_t e) {
+  if (e == cudaSuccess) return TESSA_OK;
+  return bad(e == cudaErrorMemoryAllocation ? TESSA_ERR_OOM : TESSA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
+constexpr uint64_t kMaxIds = 1ull << 31;          // sorted positions are 32-bit
+constexpr uint64_t kMaxTableRows = 0xfffffffeull;  // one key above the last row marks padding
+
+}  // namespace
+
+extern "C" {
+
+int tessa_embedding_lookup(tessa_ctx* ctx, const tessa_lookup_args* args, void* stream) {
+  if (!ctx || !args) return bad(TESSA_ERR_INVALID_ARG, "null argument");
+  const tessa_lookup_args& a = *args;
+  TRY(check_matrix("table", a.table, a.table_rows, a.dim, a.table_stride, a.dtype));
+  TRY(check_matrix("out", a.out, a.count, a.dim, a.out_stride, a.out_dtype));
+  TRY(check_ids(a.ids, a.id_bits, a.count));
+  if (a.table_rows > kMaxTableRows) return bad(TESSA_ERR_UNSUPPORTED, "table of %llu rows", (ull)a.table_rows);
+  if (a.count >= kMaxIds) return bad(TESSA_ERR_UNSUPPORTED, "%llu ids: below 2^31 are supported", (ull)a.count);
+  AsyncCtx c;
+  TRY(async_begin(ctx, &c));
+  if (a.count == 0 || a.dim == 0) return TESSA_OK;
+  return launched("embedding lookup", launch_embedding_lookup(a, c, (cudaStream_t)stream));
+}
+
+int tessa_embedding_grad_workspace(uint64_t count, uint64_t table_rows, uint32_t dim, uint64_t* bytes) {
+  if (!bytes) return bad(TESSA_ERR_INVALID_ARG, "null argument");
+  *bytes = embedding_grad_workspace(count, table_rows, dim);
+  return TESSA_OK;
+}
+
+int tessa_embedding_grad(tessa_ctx* ctx, const tessa_lookup_grad_args* args, void* workspace,
+                         uint64_t workspace_bytes, void* stream) {
+  if (!ctx || !args) return bad(TESSA_ERR_INVALID_ARG, "null argument");
+  const tessa_lookup_grad_args& a = *args;
+  TRY(check_matrix("dout", a.dout, a.count, a.dim, a.dout_stride, a.dtype));
+  TRY(check_matrix("grad", a.grad, a.table_rows, a.dim, a.grad_stride, a.grad_dtype));
+  TRY(check_ids(a.ids, a.id_bits, a.count));
+  if (a.accumulate > 1) return bad(TESSA_ERR_INVALID_ARG, "accumulate %u: 0 or 1", a.accumulate);
+  if (a.table_rows > kMaxTableRows) return bad(TESSA_ERR_UNSUPPORTED, "table of %llu rows", (ull)a.table_rows);
+  if (a.count >= kMaxIds) return bad(TESSA_ERR_UNSUPPORTED, "%llu ids: below 2^31 are supported", (ull)a.count);
+  TRY(check_workspace(workspace, workspace_bytes, embedding_grad_workspace(a.count, a.table_rows, a.dim)));
+  AsyncCtx c;
+  TRY(async_begin(ctx, &c));
+  if (a.table_rows == 0 || a.dim == 0) return TESSA_OK;
+  return launched("embedding gradient", launch_embedding_grad(a, workspace, c, (cudaStream_t)stream));
+}
+
+}  // extern "C"

@@ -2,6 +2,7 @@
 // (defined in leaf_sq8.cu, quantize_sq8.cu and assign.cu, called by capi.cu).
 #pragma once
 #include <stdint.h>
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include "../../include/tessa_sm100.h"
@@ -234,6 +235,25 @@ int submit_ring_submit(SubmitRing* ring, const tessa_subtree_request* req, uint6
 int submit_ring_poll(SubmitRing* ring, uint64_t ticket, int wait, tessa_compact_view* view);
 int submit_ring_release(SubmitRing* ring, uint64_t ticket);
 size_t reservoir_scratch_bytes(uint64_t edges, uint64_t num_points);
+
+// What the calls that only enqueue work need from a context: async_begin
+// binds its device and reports what an earlier call's kernel left in the
+// mapped error word `err`.
+struct AsyncCtx {
+  int sm_count;
+  uint64_t timeout_ns;
+  uint32_t* err;
+};
+int async_begin(tessa_ctx* ctx, AsyncCtx* out);
+
+// Training operators (embedding.cu); arguments are validated by capi_train.cu.
+cudaError_t launch_embedding_lookup(const tessa_lookup_args& a, const AsyncCtx& c, cudaStream_t stream);
+uint64_t embedding_grad_workspace(uint64_t count, uint64_t table_rows, uint32_t dim);
+cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspace, const AsyncCtx& c,
+                                  cudaStream_t stream);
+// 2-D uint8 tensor map (leaf_sq8.cu): rows x row_bytes, box of 128 bytes x
+// box_rows, 128-byte swizzle, zero fill.
+int make_code_tmap(CUtensorMap* map, const void* base, uint64_t rows, uint32_t row_bytes, uint32_t box_rows);
 
 // Records `code` and `message` as the calling thread's last error (returned by
 // tessa_last_error_message); returns `code`.

@@ -789,3 +789,132 @@ def reduce_grouped(pieces, num_points: int, l_max: int, ctx: Context | None = No
                                           _ptr(sl) if sl is not None else None, cap, ctypes.byref(count),
                                           _stream_ptr(torch, dev.index)))
     return offsets, nb, sl, int(count.value)
+
+
+# ------------------------------------------------- training the vectors
+#
+# These calls only enqueue work on the tensors' current stream.  A device-side
+# error (an id outside the table) is reported by the next of them on the
+# context or by async_status(); ids of -1 are padding.  uint32 id tensors do
+# not occur here: ids are int32 or int64.
+
+_DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
+
+
+def _dtype_code(name: str, dtype) -> int:
+    code = _DTYPES.get(str(dtype))
+    if code is None:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, not {dtype}")
+    return code
+
+
+def _matrix(name: str, t, device=None):
+    """Checks a 2-D device matrix with unit column stride; returns its row stride."""
+    if t.dim() != 2 or not t.is_cuda:
+        raise ValueError(f"{name} must be a 2-D CUDA tensor")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} must have contiguous rows (column stride 1)")
+    stride = t.stride(0) if rows > 1 else max(cols, t.stride(0))
+    if rows > 1 and cols and stride < cols:
+        raise ValueError(f"{name} has rows that overlap")
+    return stride
+
+
+def _id_tensor(ids, device):
+    import torch
+
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"ids must be int32 or int64, not {ids.dtype}")
+    if ids.device != device:
+        raise ValueError(f"ids are on {ids.device}, not on {device}")
+    return ids.contiguous(), 32 if ids.dtype == torch.int32 else 64
+
+
+def _workspace(torch, nbytes: int, device):
+    """Scratch of one call, from torch's allocator: it belongs to the current stream."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def async_status(ctx: Context | None = None, device: int = 0) -> None:
+    """Waits for the current stream and raises what the calls of this section left (tessa_async_status)."""
+    import torch
+
+    ctx = ctx or context(device)
+    C.check(C.load().tessa_async_status(ctx.handle, _stream_ptr(torch, ctx.device)))
+
+
+def embedding_lookup(table, ids, scale: float = 1.0, out=None, out_dtype=None, ctx: Context | None = None):
+    """``scale * table[ids]`` (tessa_embedding_lookup): f32 arithmetic, one rounding.
+
+    table [rows, dim] f32 / bf16 / f16 (any row stride); ids int32 or int64 of
+    any shape, -1 = padding (a row of zeros).  Returns ids.shape + (dim,) in
+    out_dtype (default the table's), or fills out [ids.numel(), dim].
+    """
+    import torch
+
+    stride = _matrix("table", table)
+    dev = table.device
+    flat, id_bits = _id_tensor(ids, dev)
+    n, dim = flat.numel(), table.shape[1]
+    if out is None:
+        res = torch.empty(ids.shape + (dim,), dtype=out_dtype or table.dtype, device=dev)
+        out, out_stride = res, dim
+    else:
+        if tuple(out.shape) != (n, dim):
+            raise ValueError(f"out has shape {tuple(out.shape)}, not {(n, dim)}")
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise ValueError(f"out is {out.dtype}, not {out_dtype}")
+        out_stride = _matrix("out", out, dev)
+        res = out
+    ctx = ctx or context(dev.index)
+    a = C.LookupArgs(table.data_ptr(), table.shape[0], stride, dim, _dtype_code("table", table.dtype),
+                     flat.data_ptr(), id_bits, _dtype_code("out", out.dtype), n, float(scale), out.data_ptr(),
+                     out_stride)
+    C.check(C.load().tessa_embedding_lookup(ctx.handle, ctypes.byref(a), _stream_ptr(torch, dev.index)))
+    return res
+
+
+def embedding_grad(dout, ids, table_rows: int, scale: float = 1.0, out_dtype=None, out=None,
+                   accumulate: bool = False, ctx: Context | None = None):
+    """Gradient of :func:`embedding_lookup` with respect to the table
+    (tessa_embedding_grad): ``grad[v] = scale * sum(dout[t] for ids[t] == v)``,
+    each row summed in f32 in the order of t, so equal inputs give equal bits.
+
+    dout [..., dim] (ids.shape + (dim,), or [ids.numel(), dim] with any row
+    stride).  Returns [table_rows, dim] in out_dtype (default dout's).  With
+    out, fills it; with accumulate, adds to it and leaves the rows that no id
+    names as they are.
+    """
+    import torch
+
+    dev = dout.device
+    dim = dout.shape[-1]
+    flat, id_bits = _id_tensor(ids, dev)
+    n = flat.numel()
+    d2 = dout if dout.dim() == 2 else dout.reshape(-1, dim)
+    if d2.shape[0] != n:
+        raise ValueError(f"dout has {d2.shape[0]} rows for {n} ids")
+    stride = _matrix("dout", d2)
+    if accumulate and out is None:
+        raise ValueError("accumulate needs out")
+    if out is None:
+        out = torch.empty((int(table_rows), dim), dtype=out_dtype or dout.dtype, device=dev)
+    elif tuple(out.shape) != (int(table_rows), dim):
+        raise ValueError(f"out has shape {tuple(out.shape)}, not {(int(table_rows), dim)}")
+    elif out_dtype is not None and out.dtype != out_dtype:
+        raise ValueError(f"out is {out.dtype}, not {out_dtype}")
+    out_stride = _matrix("out", out, dev)
+    lib = C.load()
+    need = ctypes.c_uint64()
+    C.check(lib.tessa_embedding_grad_workspace(n, out.shape[0], dim, ctypes.byref(need)))
+    ws = _workspace(torch, need.value, dev)
+    ctx = ctx or context(dev.index)
+    a = C.LookupGradArgs(d2.data_ptr(), stride, dim, _dtype_code("dout", d2.dtype), flat.data_ptr(), id_bits,
+                         _dtype_code("out", out.dtype), n, float(scale), int(bool(accumulate)), out.data_ptr(),
+                         out_stride, out.shape[0])
+    C.check(lib.tessa_embedding_grad(ctx.handle, ctypes.byref(a), _ptr(ws), need.value,
+                                     _stream_ptr(torch, dev.index)))
+    return out
