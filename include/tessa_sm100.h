@@ -739,6 +739,37 @@ TESSA_API int tessa_embedding_grad_workspace(uint64_t count, uint64_t table_rows
 TESSA_API int tessa_embedding_grad(tessa_ctx* ctx, const tessa_lookup_grad_args* args, void* workspace,
                                    uint64_t workspace_bytes, void* stream);
 
+/* Distillation from a teacher's list.  Per row t, with tau = temperature,
+ *   p = softmax(teacher_logits / tau) over the list's valid entries (id >= 0
+ *       and a logit above -inf), q = softmax(logits / tau) over all vocab,
+ *   loss = tau^2 * sum_j p_j (log p_j - log q[id_j]),
+ *   lse  = log sum exp(logits / tau),
+ *   grad[v] = row_weights[t] * tau * (q[v] - sum of p_j with id_j == v).
+ * Entries of one id add up.  A row without a valid entry, or whose logits are
+ * all -inf, takes no part: loss 0, gradient 0.  An entry whose logit is -inf
+ * while others are not makes the loss +inf, as the formula says.
+ * grad may be NULL (loss alone); it may be logits itself (same type and
+ * stride).  Statistics and sums in f32; grad rounded once to the logits' type. */
+#define TESSA_MAX_DISTILL_K 1024
+typedef struct tessa_distill_args {
+  const void* logits;           /* rows x vocab */
+  uint64_t rows;
+  uint64_t vocab;               /* below 2^32 - 1 */
+  uint64_t stride;
+  uint32_t dtype;
+  uint32_t k;                   /* 0..TESSA_MAX_DISTILL_K */
+  const void* teacher_ids;      /* rows x k, contiguous */
+  const float* teacher_logits;  /* rows x k, contiguous */
+  uint32_t id_bits;             /* 32 or 64 */
+  float temperature;            /* > 0 */
+  const float* row_weights;     /* rows, or NULL for 1 */
+  float* loss;                  /* rows, or NULL */
+  float* lse;                   /* rows, or NULL */
+  void* grad;                   /* rows x vocab, or NULL */
+  uint64_t grad_stride;
+} tessa_distill_args;
+TESSA_API int tessa_distill_topk(tessa_ctx* ctx, const tessa_distill_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -30,6 +30,7 @@ MAX_LEAF_K = 32
 MAX_RH = 4
 MAX_PADDED_DIM = 1024
 MAX_HASH_BITS = 16
+MAX_DISTILL_K = 1024
 NOALLOC_SCRATCH_BYTES = 64 << 20
 ASSIGN_FP32 = 0
 ASSIGN_SQ8 = 2
@@ -167,6 +168,15 @@ class LookupGradArgs(ctypes.Structure):
     ]
 
 
+class DistillArgs(ctypes.Structure):
+    _fields_ = [
+        ("logits", c_vp), ("rows", ctypes.c_uint64), ("vocab", ctypes.c_uint64), ("stride", ctypes.c_uint64),
+        ("dtype", ctypes.c_uint32), ("k", ctypes.c_uint32), ("teacher_ids", c_vp), ("teacher_logits", c_vp),
+        ("id_bits", ctypes.c_uint32), ("temperature", ctypes.c_float), ("row_weights", c_vp), ("loss", c_vp),
+        ("lse", c_vp), ("grad", c_vp), ("grad_stride", ctypes.c_uint64),
+    ]
+
+
 # (name, restype, argtypes) for every entry point of include/tessa_sm100.h
 SIGNATURES = [
     ("tessa_abi_version", ctypes.c_int, []),
@@ -235,6 +245,7 @@ SIGNATURES = [
     ("tessa_embedding_grad_workspace", ctypes.c_int,
      [ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint32, ctypes.POINTER(ctypes.c_uint64)]),
     ("tessa_embedding_grad", ctypes.c_int, [c_vp, ctypes.POINTER(LookupGradArgs), c_vp, ctypes.c_uint64, c_vp]),
+    ("tessa_distill_topk", ctypes.c_int, [c_vp, ctypes.POINTER(DistillArgs), c_vp]),
 ]
 
 _lib = None

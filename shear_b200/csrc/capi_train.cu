@@ -112,4 +112,24 @@ int tessa_embedding_grad(tessa_ctx* ctx, const tessa_lookup_grad_args* args, voi
   return launched("embedding gradient", launch_embedding_grad(a, workspace, c, (cudaStream_t)stream));
 }
 
+int tessa_distill_topk(tessa_ctx* ctx, const tessa_distill_args* args, void* stream) {
+  if (!ctx || !args) return bad(TESSA_ERR_INVALID_ARG, "null argument");
+  const tessa_distill_args& a = *args;
+  TRY(check_matrix("logits", a.logits, a.rows, a.vocab, a.stride, a.dtype));
+  if (a.grad) TRY(check_matrix("grad", a.grad, a.rows, a.vocab, a.grad_stride, a.dtype));
+  if (a.grad == a.logits && a.rows > 1 && a.grad_stride != a.stride)
+    return bad(TESSA_ERR_INVALID_ARG, "a gradient in place of the logits needs their stride");
+  if (a.k > TESSA_MAX_DISTILL_K) return bad(TESSA_ERR_INVALID_ARG, "list of %u entries: at most %d", a.k, TESSA_MAX_DISTILL_K);
+  if (a.vocab > kMaxTableRows) return bad(TESSA_ERR_UNSUPPORTED, "%llu logits a row", (ull)a.vocab);
+  if (a.rows > (1ull << 27)) return bad(TESSA_ERR_UNSUPPORTED, "%llu rows: at most 2^27", (ull)a.rows);
+  TRY(check_ids(a.teacher_ids, a.id_bits, a.rows * a.k));
+  if (a.rows * a.k && !a.teacher_logits) return bad(TESSA_ERR_INVALID_ARG, "teacher logits: null pointer");
+  if (!(a.temperature > 0.0f) || a.temperature > 3.0e38f)
+    return bad(TESSA_ERR_INVALID_ARG, "temperature %g: a positive number", (double)a.temperature);
+  AsyncCtx c;
+  TRY(async_begin(ctx, &c));
+  if (a.rows == 0) return TESSA_OK;
+  return launched("distillation", launch_distill(a, c, (cudaStream_t)stream));
+}
+
 }  // extern "C"

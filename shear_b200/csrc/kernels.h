@@ -246,11 +246,12 @@ struct AsyncCtx {
 };
 int async_begin(tessa_ctx* ctx, AsyncCtx* out);
 
-// Training operators (embedding.cu); arguments are validated by capi_train.cu.
+// Training operators (embedding.cu, distill.cu); arguments are validated by capi_train.cu.
 cudaError_t launch_embedding_lookup(const tessa_lookup_args& a, const AsyncCtx& c, cudaStream_t stream);
 uint64_t embedding_grad_workspace(uint64_t count, uint64_t table_rows, uint32_t dim);
 cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspace, const AsyncCtx& c,
                                   cudaStream_t stream);
+cudaError_t launch_distill(const tessa_distill_args& a, const AsyncCtx& c, cudaStream_t stream);
 // 2-D uint8 tensor map (leaf_sq8.cu): rows x row_bytes, box of 128 bytes x
 // box_rows, 128-byte swizzle, zero fill.
 int make_code_tmap(CUtensorMap* map, const void* base, uint64_t rows, uint32_t row_bytes, uint32_t box_rows);

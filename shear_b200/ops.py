@@ -918,3 +918,60 @@ def embedding_grad(dout, ids, table_rows: int, scale: float = 1.0, out_dtype=Non
     C.check(lib.tessa_embedding_grad(ctx.handle, ctypes.byref(a), _ptr(ws), need.value,
                                      _stream_ptr(torch, dev.index)))
     return out
+
+
+def _distill(logits, teacher_ids, teacher_logits, temperature, row_weights, want_stats, want_grad, out, ctx):
+    import torch
+
+    stride = _matrix("logits", logits)
+    dev = logits.device
+    rows, vocab = logits.shape
+    if teacher_ids.dim() != 2 or teacher_ids.shape[0] != rows or teacher_logits.shape != teacher_ids.shape:
+        raise ValueError(f"teacher_ids {tuple(teacher_ids.shape)} and teacher_logits {tuple(teacher_logits.shape)} "
+                         f"must both be [{rows}, k]")
+    ids, id_bits = _id_tensor(teacher_ids, dev)
+    if not teacher_logits.is_floating_point() or teacher_logits.device != dev:
+        raise ValueError("teacher_logits must be floating point and on the logits' device")
+    tl = teacher_logits.to(torch.float32).contiguous()
+    if row_weights is not None:
+        if tuple(row_weights.shape) != (rows,) or row_weights.device != dev:
+            raise ValueError(f"row_weights must be [{rows}] on the logits' device")
+        row_weights = row_weights.to(torch.float32).contiguous()
+    loss = torch.empty(rows, dtype=torch.float32, device=dev) if want_stats else None
+    lse = torch.empty(rows, dtype=torch.float32, device=dev) if want_stats else None
+    grad, grad_stride = None, 0
+    if want_grad:
+        grad = torch.empty((rows, vocab), dtype=logits.dtype, device=dev) if out is None else out
+        if tuple(grad.shape) != (rows, vocab) or grad.dtype != logits.dtype:
+            raise ValueError(f"out must be {(rows, vocab)} of {logits.dtype}")
+        grad_stride = _matrix("out", grad, dev)
+    ctx = ctx or context(dev.index)
+    a = C.DistillArgs(logits.data_ptr(), rows, vocab, stride, _dtype_code("logits", logits.dtype), ids.shape[1],
+                      ids.data_ptr(), tl.data_ptr(), id_bits, float(temperature), _ptr(row_weights).value,
+                      _ptr(loss).value, _ptr(lse).value, _ptr(grad).value, grad_stride)
+    C.check(C.load().tessa_distill_topk(ctx.handle, ctypes.byref(a), _stream_ptr(torch, dev.index)))
+    return loss, lse, grad
+
+
+def distill_topk(logits, teacher_ids, teacher_logits, temperature: float = 1.0, ctx: Context | None = None):
+    """Distillation loss from a teacher's list, per row (tessa_distill_topk).
+
+    logits [rows, vocab] f32 / bf16 / f16; teacher_ids [rows, k] int32 or
+    int64 (-1 = no entry) and teacher_logits [rows, k], k <= 1024.  With
+    p = softmax of the list at the temperature and q = softmax(logits /
+    temperature) over the whole row, returns (loss f32 [rows], temperature^2 *
+    KL(p || q), and lse f32 [rows], log-sum-exp of logits / temperature).
+    """
+    loss, lse, _ = _distill(logits, teacher_ids, teacher_logits, temperature, None, True, False, None, ctx)
+    return loss, lse
+
+
+def distill_topk_grad(logits, teacher_ids, teacher_logits, temperature: float = 1.0, row_weights=None, out=None,
+                      ctx: Context | None = None):
+    """:func:`distill_topk` and, from the same read of the logits, the gradient
+    of sum(row_weights * loss) with respect to them.
+
+    Returns (loss, lse, grad [rows, vocab] in the logits' type).  out receives
+    the gradient; it may be the logits themselves.
+    """
+    return _distill(logits, teacher_ids, teacher_logits, temperature, row_weights, True, True, out, ctx)
