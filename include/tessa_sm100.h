@@ -739,6 +739,51 @@ TESSA_API int tessa_embedding_grad_workspace(uint64_t count, uint64_t table_rows
 TESSA_API int tessa_embedding_grad(tessa_ctx* ctx, const tessa_lookup_grad_args* args, void* workspace,
                                    uint64_t workspace_bytes, void* stream);
 
+/* FP8 codes with a scale for each block of 128 consecutive values of a row:
+ * the scale is the least power of two s with max|x| / s <= 448, kept as its
+ * biased exponent (E8M0: s = 2^(byte - 127); 0 for a block of zeros), and the
+ * code is x / s rounded to E4M3, ties to even.  A NaN or infinite value
+ * becomes the NaN code and takes no part in its block's scale.  For cols
+ * columns, a row of codes has fp8_cols = cols rounded up to 16 bytes (zeros
+ * past cols), a row of scales fp8_scales = 4 * ceil(cols / 512) bytes (zeros
+ * past the last block).  codes / scales: x's rows; codes_t / scales_t: x's
+ * columns (cols rows of `rows` values, blocks of 128 down a column).  Either
+ * pair may be NULL. */
+typedef struct tessa_fp8_quantize_args {
+  const void* x;                /* rows x cols */
+  uint64_t rows;
+  uint64_t cols;
+  uint64_t stride;
+  uint32_t dtype;
+  uint32_t reserved;
+  uint8_t* codes;               /* rows x (cols rounded up to 16), 16-byte aligned */
+  uint8_t* scales;              /* rows x 4 * ceil(cols / 512) */
+  uint8_t* codes_t;             /* cols x (rows rounded up to 16), 16-byte aligned */
+  uint8_t* scales_t;            /* cols x 4 * ceil(rows / 512) */
+} tessa_fp8_quantize_args;
+TESSA_API int tessa_quantize_fp8(tessa_ctx* ctx, const tessa_fp8_quantize_args* args, void* stream);
+
+/* out[m][n] = sum over blocks of sa * sb * (a . b): a is m x k codes, b n x k
+ * codes in the layout above (k a multiple of 16), products summed in f32 on
+ * the tensor cores and rounded once to out's type. */
+typedef struct tessa_fp8_matmul_args {
+  const uint8_t* a_codes;
+  const uint8_t* a_scales;
+  const uint8_t* b_codes;
+  const uint8_t* b_scales;
+  uint64_t m;
+  uint64_t n;
+  uint64_t k;
+  void* out;                    /* m x n */
+  uint64_t out_stride;
+  uint32_t out_dtype;
+  uint32_t reserved;
+} tessa_fp8_matmul_args;
+/* Scratch of a product of this shape on this context's device; may be 0. */
+TESSA_API int tessa_matmul_fp8_workspace(tessa_ctx* ctx, uint64_t m, uint64_t n, uint64_t k, uint64_t* bytes);
+TESSA_API int tessa_matmul_fp8(tessa_ctx* ctx, const tessa_fp8_matmul_args* args, void* workspace,
+                               uint64_t workspace_bytes, void* stream);
+
 /* Distillation from a teacher's list.  Per row t, with tau = temperature,
  *   p = softmax(teacher_logits / tau) over the list's valid entries (id >= 0
  *       and a logit above -inf), q = softmax(logits / tau) over all vocab,

@@ -168,6 +168,22 @@ class LookupGradArgs(ctypes.Structure):
     ]
 
 
+class Fp8QuantizeArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_vp), ("rows", ctypes.c_uint64), ("cols", ctypes.c_uint64), ("stride", ctypes.c_uint64),
+        ("dtype", ctypes.c_uint32), ("reserved", ctypes.c_uint32), ("codes", c_vp), ("scales", c_vp),
+        ("codes_t", c_vp), ("scales_t", c_vp),
+    ]
+
+
+class Fp8MatmulArgs(ctypes.Structure):
+    _fields_ = [
+        ("a_codes", c_vp), ("a_scales", c_vp), ("b_codes", c_vp), ("b_scales", c_vp), ("m", ctypes.c_uint64),
+        ("n", ctypes.c_uint64), ("k", ctypes.c_uint64), ("out", c_vp), ("out_stride", ctypes.c_uint64),
+        ("out_dtype", ctypes.c_uint32), ("reserved", ctypes.c_uint32),
+    ]
+
+
 class DistillArgs(ctypes.Structure):
     _fields_ = [
         ("logits", c_vp), ("rows", ctypes.c_uint64), ("vocab", ctypes.c_uint64), ("stride", ctypes.c_uint64),
@@ -246,6 +262,10 @@ SIGNATURES = [
      [ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint32, ctypes.POINTER(ctypes.c_uint64)]),
     ("tessa_embedding_grad", ctypes.c_int, [c_vp, ctypes.POINTER(LookupGradArgs), c_vp, ctypes.c_uint64, c_vp]),
     ("tessa_distill_topk", ctypes.c_int, [c_vp, ctypes.POINTER(DistillArgs), c_vp]),
+    ("tessa_quantize_fp8", ctypes.c_int, [c_vp, ctypes.POINTER(Fp8QuantizeArgs), c_vp]),
+    ("tessa_matmul_fp8_workspace", ctypes.c_int,
+     [c_vp, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint64, ctypes.POINTER(ctypes.c_uint64)]),
+    ("tessa_matmul_fp8", ctypes.c_int, [c_vp, ctypes.POINTER(Fp8MatmulArgs), c_vp, ctypes.c_uint64, c_vp]),
 ]
 
 _lib = None

@@ -763,6 +763,8 @@ int assign_device(tessa_ctx* ctx, uint32_t source, const tessa_assign_args* a, c
 
 }  // namespace
 
+int tessa::ctx_sm_count(const tessa_ctx* ctx) { return ctx->sm_count; }
+
 int tessa::async_begin(tessa_ctx* ctx, AsyncCtx* out) {
   TRY(bind(ctx));
   if (!ctx->async_err) {

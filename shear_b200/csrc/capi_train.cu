@@ -69,6 +69,7 @@ int launched(const char* what, cudaError_t e) {
 }
 
 constexpr uint64_t kMaxIds = 1ull << 31;          // sorted positions are 32-bit
+constexpr uint64_t kMaxMatrix = (1ull << 31) - 1;  // TMA coordinates and tile counts are 32-bit
 constexpr uint64_t kMaxTableRows = 0xfffffffeull;  // one key above the last row marks padding
 
 }  // namespace
@@ -110,6 +111,57 @@ int tessa_embedding_grad(tessa_ctx* ctx, const tessa_lookup_grad_args* args, voi
   TRY(async_begin(ctx, &c));
   if (a.table_rows == 0 || a.dim == 0) return TESSA_OK;
   return launched("embedding gradient", launch_embedding_grad(a, workspace, c, (cudaStream_t)stream));
+}
+
+int tessa_quantize_fp8(tessa_ctx* ctx, const tessa_fp8_quantize_args* args, void* stream) {
+  if (!ctx || !args) return bad(TESSA_ERR_INVALID_ARG, "null argument");
+  const tessa_fp8_quantize_args& a = *args;
+  TRY(check_matrix("x", a.x, a.rows, a.cols, a.stride, a.dtype));
+  if (a.rows > kMaxMatrix || a.cols > kMaxMatrix)
+    return bad(TESSA_ERR_UNSUPPORTED, "matrix of %llu x %llu: both below 2^31", (ull)a.rows, (ull)a.cols);
+  if ((a.rows + 127) / 128 * ((a.cols + 127) / 128) > kMaxMatrix)
+    return bad(TESSA_ERR_UNSUPPORTED, "matrix of %llu x %llu is too large", (ull)a.rows, (ull)a.cols);
+  if (!a.codes != !a.scales || !a.codes_t != !a.scales_t || (!a.codes && !a.codes_t)) {
+    if (a.rows && a.cols) return bad(TESSA_ERR_INVALID_ARG, "codes and scales come in pairs, one pair at least");
+  }
+  if (reinterpret_cast<uintptr_t>(a.codes) % 16 || reinterpret_cast<uintptr_t>(a.codes_t) % 16)
+    return bad(TESSA_ERR_INVALID_ARG, "codes must start on a 16-byte boundary");
+  AsyncCtx c;
+  TRY(async_begin(ctx, &c));
+  if (a.rows == 0 || a.cols == 0) return TESSA_OK;
+  return launched("FP8 quantizer", launch_quantize_fp8(a, c, (cudaStream_t)stream));
+}
+
+int tessa_matmul_fp8_workspace(tessa_ctx* ctx, uint64_t m, uint64_t n, uint64_t k, uint64_t* bytes) {
+  if (!ctx || !bytes) return bad(TESSA_ERR_INVALID_ARG, "null argument");
+  if (m > kMaxMatrix || n > kMaxMatrix || k > kMaxMatrix)
+    return bad(TESSA_ERR_UNSUPPORTED, "product of %llu x %llu x %llu: each below 2^31", (ull)m, (ull)n, (ull)k);
+  *bytes = fp8_matmul_workspace(m, n, k, ctx_sm_count(ctx));
+  return TESSA_OK;
+}
+
+int tessa_matmul_fp8(tessa_ctx* ctx, const tessa_fp8_matmul_args* args, void* workspace, uint64_t workspace_bytes,
+                     void* stream) {
+  if (!ctx || !args) return bad(TESSA_ERR_INVALID_ARG, "null argument");
+  const tessa_fp8_matmul_args& a = *args;
+  TRY(check_matrix("out", a.out, a.m, a.n, a.out_stride, a.out_dtype));
+  uint64_t need = 0;
+  TRY(tessa_matmul_fp8_workspace(ctx, a.m, a.n, a.k, &need));
+  if (a.k % 16) return bad(TESSA_ERR_INVALID_ARG, "k=%llu: rows of codes are a multiple of 16", (ull)a.k);
+  if ((a.m + 15) / 16 * ((a.n + 127) / 128) > kMaxMatrix / 32)
+    return bad(TESSA_ERR_UNSUPPORTED, "product of %llu x %llu is too large", (ull)a.m, (ull)a.n);
+  if (a.m && a.n && a.k) {
+    if (!a.a_codes || !a.a_scales || !a.b_codes || !a.b_scales) return bad(TESSA_ERR_INVALID_ARG, "null codes or scales");
+    if (reinterpret_cast<uintptr_t>(a.a_codes) % 16 || reinterpret_cast<uintptr_t>(a.b_codes) % 16)
+      return bad(TESSA_ERR_INVALID_ARG, "codes must start on a 16-byte boundary");
+    if (reinterpret_cast<uintptr_t>(a.a_scales) % 4 || reinterpret_cast<uintptr_t>(a.b_scales) % 4)
+      return bad(TESSA_ERR_INVALID_ARG, "scales must start on a 4-byte boundary");
+  }
+  TRY(check_workspace(workspace, workspace_bytes, need));
+  AsyncCtx c;
+  TRY(async_begin(ctx, &c));
+  if (a.m == 0 || a.n == 0) return TESSA_OK;
+  return launched("FP8 product", launch_matmul_fp8(a, workspace, c, (cudaStream_t)stream));
 }
 
 int tessa_distill_topk(tessa_ctx* ctx, const tessa_distill_args* args, void* stream) {

@@ -920,6 +920,93 @@ def embedding_grad(dout, ids, table_rows: int, scale: float = 1.0, out_dtype=Non
     return out
 
 
+def _fp8_shape(rows: int, cols: int):
+    """Shapes of the codes and scales of `rows` rows of `cols` values."""
+    return (rows, (cols + 15) // 16 * 16), (rows, (cols + 511) // 512 * 4)
+
+
+def _quantize_fp8(x, along_rows: bool, along_cols: bool, ctx):
+    import torch
+
+    stride = _matrix("x", x)
+    dev = x.device
+    rows, cols = x.shape
+    res = []
+    for wanted, shape in ((along_rows, (rows, cols)), (along_cols, (cols, rows))):
+        if wanted:
+            c, s = _fp8_shape(*shape)
+            res += [torch.empty(c, dtype=torch.float8_e4m3fn, device=dev), torch.empty(s, dtype=torch.uint8, device=dev)]
+        else:
+            res += [None, None]
+    ctx = ctx or context(dev.index)
+    a = C.Fp8QuantizeArgs(x.data_ptr(), rows, cols, stride, _dtype_code("x", x.dtype), 0, *(_ptr(t).value for t in res))
+    C.check(C.load().tessa_quantize_fp8(ctx.handle, ctypes.byref(a), _stream_ptr(torch, dev.index)))
+    return res
+
+
+def quantize_fp8(x, transpose: bool = False, ctx: Context | None = None):
+    """FP8 (E4M3) codes with a power-of-two scale per block of 128 (tessa_quantize_fp8).
+
+    x [rows, cols] f32 / bf16 / f16, any row stride.  Returns (codes
+    float8_e4m3fn [rows, cols rounded up to 16], scales uint8 [rows, 4 *
+    ceil(cols / 512)]): block b of a row stands for codes * 2^(scale - 127).
+    With transpose, the codes of x's columns: [cols, rows rounded up to 16],
+    blocks down the columns.
+    """
+    res = _quantize_fp8(x, not transpose, transpose, ctx)
+    return tuple(res[2:] if transpose else res[:2])
+
+
+def quantize_fp8_both(x, ctx: Context | None = None):
+    """(codes, scales, codes_t, scales_t): both forms of :func:`quantize_fp8`
+    from one read of x, as a product and its gradients need them."""
+    return tuple(_quantize_fp8(x, True, True, ctx))
+
+
+def _fp8_operand(name: str, codes, scales):
+    import torch
+
+    if codes.dtype not in (torch.float8_e4m3fn, torch.uint8) or scales.dtype != torch.uint8:
+        raise ValueError(f"{name}: codes must be float8_e4m3fn (or its bytes) and scales uint8")
+    if codes.dim() != 2 or not codes.is_cuda or not codes.is_contiguous() or not scales.is_contiguous():
+        raise ValueError(f"{name}: codes and scales must be contiguous 2-D CUDA tensors")
+    want = _fp8_shape(codes.shape[0], codes.shape[1])
+    if tuple(codes.shape) != want[0] or tuple(scales.shape) != want[1] or scales.device != codes.device:
+        raise ValueError(f"{name}: scales {tuple(scales.shape)} do not fit codes {tuple(codes.shape)}")
+
+
+def matmul_fp8(a_codes, a_scales, b_codes, b_scales, out_dtype=None, out=None, ctx: Context | None = None):
+    """``out[m, n] = sum_k a[m, k] * b[n, k]`` over FP8 codes with block scales
+    (tessa_matmul_fp8): summed in f32, rounded once.
+
+    Operands as :func:`quantize_fp8` returns them, of the same width.  Returns
+    [m, n] in out_dtype (default float32), or fills out (any row stride).
+    """
+    import torch
+
+    _fp8_operand("a", a_codes, a_scales)
+    _fp8_operand("b", b_codes, b_scales)
+    dev = a_codes.device
+    m, k = a_codes.shape
+    n = b_codes.shape[0]
+    if b_codes.shape[1] != k or b_codes.device != dev:
+        raise ValueError(f"operands of {tuple(a_codes.shape)} on {dev} and {tuple(b_codes.shape)} on {b_codes.device}")
+    if out is None:
+        out = torch.empty((m, n), dtype=out_dtype or torch.float32, device=dev)
+    elif tuple(out.shape) != (m, n) or (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError(f"out must be {(m, n)}" + (f" of {out_dtype}" if out_dtype is not None else ""))
+    out_stride = _matrix("out", out, dev)
+    lib = C.load()
+    ctx = ctx or context(dev.index)
+    need = ctypes.c_uint64()
+    C.check(lib.tessa_matmul_fp8_workspace(ctx.handle, m, n, k, ctypes.byref(need)))
+    ws = _workspace(torch, need.value, dev)
+    a = C.Fp8MatmulArgs(a_codes.data_ptr(), a_scales.data_ptr(), b_codes.data_ptr(), b_scales.data_ptr(), m, n, k,
+                        out.data_ptr(), out_stride, _dtype_code("out", out.dtype), 0)
+    C.check(lib.tessa_matmul_fp8(ctx.handle, ctypes.byref(a), _ptr(ws), need.value, _stream_ptr(torch, dev.index)))
+    return out
+
+
 def _distill(logits, teacher_ids, teacher_logits, temperature, row_weights, want_stats, want_grad, out, ctx):
     import torch
 
