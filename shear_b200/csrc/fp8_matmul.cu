@@ -7,13 +7,16 @@
 // sum over K never leaves the f32 accumulator in tensor memory: no pass over
 // the accumulator per block, as a free f32 scale would need.
 //
-// One persistent CTA per SM; the roles run concurrently:
-//   warp 0    TMA: stages of 128 bytes of K: 128 rows of b, BN rows of a
-//   warp 1    tensor memory, scales' copies into it (tcgen05.cp), MMAs
-//   warp 2    scales: 32-bit words (four blocks of K) from global to shared
-//             memory, in the order tcgen05.cp wants
-//   warps 4-7 epilogue: accumulators to global memory
-// b's rows are the accumulator's 128 lanes and a's rows its columns, so a warp
+// Persistent pairs of CTAs (two SMs) share a tile of 256 rows of b and BN rows
+// of a: each CTA holds 128 rows of b and half of a's in shared memory, and one
+// MMA (cta_group::2) reads both halves, so a stage brings 31 KB into an SM
+// where a CTA alone would need 47 KB for the same work.  Roles, concurrently:
+//   warp 0      TMA: stages of 128 bytes of K
+//   warp 1      tensor memory; in the first CTA the pair's MMAs
+//   warps 4-7   scales: 32-bit words (four blocks of K) from global memory to
+//               the four lane quadrants of tensor memory
+//   warps 8-15  epilogue: accumulators to global memory
+// b's rows are the accumulator's lanes and a's rows its columns, so a warp
 // holds 32 consecutive n of one m and stores them straight to out, and a batch
 // of few rows makes a narrow MMA (BN from 16) instead of a mostly empty one.
 // Two accumulators: one is emptied while the next is summed.
@@ -27,15 +30,15 @@ namespace tessa {
 namespace train {
 namespace mm {
 
-constexpr uint32_t kThreads = 256;
-constexpr uint32_t kBP = 128;             // rows of b a tile (accumulator lanes)
-constexpr uint32_t kMaxBN = 240;          // rows of a a tile: two accumulators and the scales fit 512 columns
+constexpr uint32_t kThreads = 512;
+constexpr uint32_t kBP = 128;             // rows of b a CTA (accumulator lanes)
+constexpr uint32_t kMaxBN = 224;          // rows of a a tile: two accumulators leave 64 of 512 columns to the scales
 constexpr uint32_t kBK = 128;             // bytes of K a stage
-constexpr uint32_t kScaleBufs = 4;        // shared memory buffers of scale words
-constexpr uint32_t kScaleBytes = 512 + 1024;  // 128 words of b, up to 256 of a
-constexpr uint32_t kScaleCol = 480;       // tensor memory columns of the scales: two sets of 16
+constexpr uint32_t kScaleCol = 448;       // tensor memory columns of the scales
+constexpr uint32_t kSets = 4;             // sets of 16: the scale warps run up to three groups ahead
 constexpr uint32_t kMaxStages = 10;
 constexpr uint32_t kSmemLimit = 227u * 1024u;
+constexpr uint32_t kScaleWarp = 4, kEpiWarp = 8;
 
 struct Params {
   const uint8_t* p_scales;  // b's
@@ -58,7 +61,7 @@ struct Params {
 // kind::mxf8f6f4, E4M3 x E4M3, both K-major, E8M0 scales, f32 accumulators;
 // scale_id selects the byte of the scale words.
 __device__ __forceinline__ uint32_t idesc_mx(uint32_t bn, uint32_t scale_id) {
-  return (scale_id << 4) | ((bn >> 3) << 17) | (1u << 23) | ((kBP >> 4) << 24) | (scale_id << 29);
+  return (scale_id << 4) | ((bn >> 3) << 17) | (1u << 23) | ((2u * kBP >> 4) << 24) | (scale_id << 29);
 }
 
 __device__ __forceinline__ void mma_mx(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa,
@@ -66,15 +69,8 @@ __device__ __forceinline__ void mma_mx(uint32_t d, uint64_t adesc, uint64_t bdes
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate));
-}
-
-// 32 rows x 16 bytes of shared memory (unswizzled, rows 16 bytes apart) to
-// four tensor memory columns, repeated in the four lane quadrants.
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t smem_addr) {
-  const uint64_t desc = (uint64_t)((smem_addr >> 4) & 0x3FFFu) | (uint64_t)(128u >> 4) << 32 | (uint64_t)1u << 46;
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
 __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -84,6 +80,80 @@ __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_st_x4(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0u;
+}
+
+// Arrives on the barrier at this offset in both CTAs once the MMAs issued so far have completed.
+__device__ __forceinline__ void commit_both(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+// Arrives on a barrier of either CTA.  What the pair's barriers guard is
+// tensor memory, ordered by tcgen05.fence, and shared memory that TMA writes:
+// no ordinary memory, so a release at cluster scope, which waits for the
+// thread's loads and stores in flight (2000 cycles here), is not needed.
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+__device__ __forceinline__ void expect_at(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+// TMA tile load into this CTA whose bytes complete on a barrier of the pair (no multicast).
+__device__ __forceinline__ void load_at(const CUtensorMap* map, uint32_t dst, uint32_t bar, int32_t x, int32_t y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+
+__device__ __forceinline__ bool try_at(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0u;
+}
+// mbar_wait by shared-memory address; the first look costs a few instructions.
+__device__ __forceinline__ bool wait_at(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t* err,
+                                        uint64_t timeout_ns) {
+  return try_at(bar, parity) || mbar_wait(reinterpret_cast<uint64_t*>(__cvta_shared_to_generic(bar)), parity,
+                                          abort_flag, err, timeout_ns);
+}
+
+// Barrier of the four scale warps; whether any thread said so.
+__device__ __forceinline__ bool meet_any(bool said) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(said ? 1u : 0u)
+      : "memory");
+  return r != 0u;
 }
 
 struct Unit {
@@ -107,35 +177,67 @@ __device__ __forceinline__ Unit unit_of(const Params& p, uint32_t u) {
   r.kb1 = min(p.kblocks, r.kb0 + p.split_groups * 4u);
   return r;
 }
+// The blocks of K alone: all that the MMA warp needs, without the divisions
+// that would leave the tensor core idle between tiles.
+__device__ __forceinline__ void span_of(const Params& p, uint32_t u, uint32_t& kb0, uint32_t& kb1) {
+  kb0 = 0;
+  kb1 = p.kblocks;
+  if (p.splits > 1u) {
+    kb0 = u % p.splits * p.split_groups * 4u;
+    kb1 = min(p.kblocks, kb0 + p.split_groups * 4u);
+  }
+}
+
+// Sixteen accumulator columns of the lane's row: out[i * stride], i < rows.
+template <class O>
+__device__ __forceinline__ void store16(O* out, uint64_t stride, const uint32_t (&v)[16], uint32_t rows) {
+  if (rows >= 16u) {
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) {
+      *out = from_f32<O>(__uint_as_float(v[i]));
+      out += stride;
+    }
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) {
+      if (i < rows) *out = from_f32<O>(__uint_as_float(v[i]));
+      out += stride;
+    }
+  }
+}
 
 template <class O, bool PARTS>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fp8_matmul_kernel(const __grid_constant__ CUtensorMap pmap, const __grid_constant__ CUtensorMap qmap,
                       const Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~(uintptr_t)1023u);
-  __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], sf_full[kScaleBufs], sf_empty[kScaleBufs],
-      acc_full[2], acc_empty[2], group_done[2], drained;
+  // In the first CTA: full, scale_full and acc_empty count both CTAs' work.
+  // The other barriers are signalled in both CTAs.
+  __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], scale_full[kSets], group_done[kSets],
+      acc_full[2], acc_empty[2], drained;
+  __shared__ uint32_t scale_words[2][kBP + 256];  // a group's words: b's rows, a's rows
   __shared__ uint32_t tmem_slot, abort_word;
   volatile uint32_t* abort_flag = &abort_word;
   const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
-  const uint32_t stage_bytes = (kBP + p.bn) * kBK;
-  uint8_t* scales = smem + p.stages * stage_bytes;
+  const uint32_t rank = cluster_ctarank();
+  const uint32_t half_bn = p.bn / 2u;
+  const uint32_t stage_bytes = (kBP + half_bn) * kBK;  // of one CTA
   const uint32_t units = p.tiles_p * p.tiles_q * p.splits;
+  const uint32_t unit0 = blockIdx.x / 2u, ustep = gridDim.x / 2u;
 
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < kMaxStages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (uint32_t i = 0; i < kScaleBufs; ++i) {
-      mbar_init(&sf_full[i], 1);
-      mbar_init(&sf_empty[i], 1);
+    for (uint32_t i = 0; i < kSets; ++i) {
+      mbar_init(&scale_full[i], 8);
+      mbar_init(&group_done[i], 1);
     }
     for (uint32_t i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 4);
-      mbar_init(&group_done[i], 1);
+      mbar_init(&acc_empty[i], 16);
     }
     mbar_init(&drained, 1);
     abort_word = 0u;
@@ -147,11 +249,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&qmap);
   }
   if (warp == 1) {
-    tmem_alloc(&tmem_slot, 512);
-    tmem_relinquish();
+    tmem_alloc_pair(&tmem_slot, 512);
+    tmem_relinquish_pair();
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync();  // the peer's barriers are initialised before any arrival on them
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -159,122 +262,196 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
 
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t it = 0;  // stages filled so far
-      bool ok = true;
-      for (uint32_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
-        const Unit t = unit_of(p, u);
-        for (uint32_t kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-          const uint32_t s = it % p.stages;
-          if (!wait(&empty[s], ((it / p.stages) & 1u) ^ 1u)) {
-            ok = false;
-            break;
-          }
-          mbar_arrive_expect_tx(&full[s], stage_bytes);
-          uint8_t* dst = smem + s * stage_bytes;
-          tma_load_2d(&pmap, dst, &full[s], (int32_t)(kb * kBK), (int32_t)(t.p * kBP));
-          tma_load_2d(&qmap, dst + kBP * kBK, &full[s], (int32_t)(kb * kBK), (int32_t)(t.q * p.bn));
+    const bool one = elect_one();
+    const uint32_t ring = smem_u32(smem), empty_base = smem_u32(empty), full_base = smem_u32(full);
+    const uint32_t full_first = mapa_shared(full, 0);  // both CTAs' bytes complete on the first CTA's barrier
+    uint32_t s = 0, phase = 0, filled = 0;
+    bool ok = true;
+    for (uint32_t u = unit0; u < units && ok; u += ustep) {
+      const Unit t = unit_of(p, u);
+      const int32_t py = (int32_t)((t.p * 2u + rank) * kBP), qy = (int32_t)(t.q * p.bn + rank * half_bn);
+      for (uint32_t kb = t.kb0; kb < t.kb1; ++kb) {
+        ok &= wait_at(empty_base + s * 8u, phase ^ 1u, abort_flag, p.err, p.timeout_ns);
+        if (one && ok) {
+          if (rank == 0) expect_at(full_base + s * 8u, 2u * stage_bytes);
+          const uint32_t dst = ring + s * stage_bytes, bar = full_first + s * 8u;
+          load_at(&pmap, dst, bar, (int32_t)(kb * kBK), py);
+          load_at(&qmap, dst + kBP * kBK, bar, (int32_t)(kb * kBK), qy);
+        }
+        __syncwarp();
+        filled += ok ? 1u : 0u;
+        if (++s == p.stages) {
+          s = 0;
+          phase ^= 1u;
         }
       }
-      // The block may not end before its copies have landed.
-      uint32_t dummy = 0u;
-      for (uint32_t i = it > p.stages ? it - p.stages : 0u; i < it; ++i)
-        mbar_wait(&full[i % p.stages], (i / p.stages) & 1u, &dummy, p.err, p.timeout_ns);
+      ok = __all_sync(0xffffffffu, ok);
     }
+    // The block may not end before its copies have landed.  The first CTA sees
+    // both CTAs' bytes; after a wait gave up somewhere the other, whose copies
+    // may lack their counterpart, leaves them ample time instead.
+    if (lane == 0 && rank == 0) {
+      uint32_t dummy = 0u;
+      for (uint32_t i = filled > p.stages ? filled - p.stages : 0u; i < filled; ++i)
+        mbar_wait(&full[i % p.stages], (i / p.stages) & 1u, &dummy, p.err, p.timeout_ns);
+    } else if (lane == 0 && !ok) {
+      const uint64_t t0 = global_timer_ns();
+      while (global_timer_ns() - t0 < 1000000ull) __nanosleep(1000);
+    }
+    __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t base = smem_u32(smem), scale_base = smem_u32(scales);
-      uint32_t it = 0, group = 0, acc = 0;
+    if (rank == 1) {
+      // The pair's MMAs read this CTA's memory until they have all completed.
+      uint32_t dummy = 0u;
+      if (lane == 0) mbar_wait(&drained, 0u, &dummy, p.err, p.timeout_ns);
+    } else {
+      // The warp stays together, every operand of an MMA is the same in all
+      // lanes and no branch depends on a wait's answer, so that the compiler
+      // keeps the operands in uniform registers: an issue from one diverged
+      // lane costs over 100 cycles, as much as an MMA.  After a wait that gave
+      // up the tile's remaining MMAs therefore still run, on whatever the
+      // stages hold, and the loop ends with the tile.
+      const bool one = elect_one();
+      const uint64_t base = smem_desc_sw128(smem_u32(smem));
+      const uint32_t full_base = smem_u32(full), empty_base = smem_u32(empty);
+      const uint32_t desc_step = stage_bytes >> 4;
+      const uint32_t whole = p.ksteps / 4u;  // blocks before the one that K may end inside
+      uint32_t s = 0, phase = 0, group = 0, acc = 0;
       bool ok = true;
-      for (uint32_t u = blockIdx.x; u < units && ok; u += gridDim.x, ++acc) {
-        const Unit t = unit_of(p, u);
+      for (uint32_t u = unit0; u < units && ok; u += ustep, ++acc) {
+        uint32_t kb0, kb1;
+        span_of(p, u, kb0, kb1);
         const uint32_t buf = acc & 1u;
-        if (!wait(&acc_empty[buf], ((acc >> 1) & 1u) ^ 1u)) break;
-        tc_fence_after();
+        ok &= wait_at(smem_u32(&acc_empty[buf]), ((acc >> 1) & 1u) ^ 1u, abort_flag, p.err, p.timeout_ns);
         const uint32_t d = tmem + buf * kMaxBN;
-        for (uint32_t kb = t.kb0; kb < t.kb1 && ok; kb += 4u, ++group) {
-          // The group's scales: into the tensor memory set that the group
-          // before the last has finished reading.
-          const uint32_t sb = group % kScaleBufs, set = group & 1u;
+        uint32_t accumulate = 0;
+        for (uint32_t kb = kb0; kb < kb1; kb += 4u, ++group) {
+          const uint32_t set = group % kSets;
           const uint32_t sfp = tmem + kScaleCol + set * 16u, sfq = sfp + 4u;
-          if (!wait(&sf_full[sb], (group / kScaleBufs) & 1u) ||
-              (group >= 2u && !wait(&group_done[set], ((group >> 1) - 1u) & 1u))) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t sa = scale_base + sb * kScaleBytes;
-          copy_scales(sfp, sa);
-          copy_scales(sfq, sa + 512u);
-          if (p.bn > 128u) copy_scales(sfq + 4u, sa + 1024u);
-          mma_commit(&sf_empty[sb]);
-          const uint32_t end = min(kb + 4u, t.kb1);
-          for (uint32_t b = kb; b < end; ++b, ++it) {
-            const uint32_t s = it % p.stages;
-            if (!wait(&full[s], (it / p.stages) & 1u)) {
-              ok = false;
-              break;
-            }
+          ok &= wait_at(smem_u32(&scale_full[set]), (group / kSets) & 1u, abort_flag, p.err, p.timeout_ns);
+          const uint32_t end = min(kb + 4u, kb1), full_end = min(end, whole);
+          uint32_t idesc = idesc_mx(p.bn, 0), b = kb;
+          for (; b < full_end; ++b, idesc += idesc_mx(0, 1) - idesc_mx(0, 0)) {
+            ok &= wait_at(full_base + s * 8u, phase, abort_flag, p.err, p.timeout_ns);
             tc_fence_after();
-            const uint32_t pa = base + s * stage_bytes, qa = pa + kBP * kBK;
-            const uint32_t idesc = idesc_mx(p.bn, b - kb);
-            const uint32_t steps = min(4u, p.ksteps - b * 4u);
-            for (uint32_t k = 0; k < steps; ++k)
-              mma_mx(d, smem_desc_sw128(pa + k * 32u), smem_desc_sw128(qa + k * 32u), idesc, sfp, sfq,
-                     b > t.kb0 || k > 0u ? 1u : 0u);
-            mma_commit(&empty[s]);
+            const uint64_t pd = base + s * desc_step, qd = pd + (kBP * kBK >> 4);
+            if (one) {
+              mma_mx(d, pd, qd, idesc, sfp, sfq, accumulate);
+              mma_mx(d, pd + 2u, qd + 2u, idesc, sfp, sfq, 1u);
+              mma_mx(d, pd + 4u, qd + 4u, idesc, sfp, sfq, 1u);
+              mma_mx(d, pd + 6u, qd + 6u, idesc, sfp, sfq, 1u);
+              commit_both(empty_base + s * 8u);
+            }
+            __syncwarp();
+            accumulate = 1u;
+            if (++s == p.stages) {
+              s = 0;
+              phase ^= 1u;
+            }
           }
-          if (ok) mma_commit(&group_done[set]);
+          if (b < end) {
+            ok &= wait_at(full_base + s * 8u, phase, abort_flag, p.err, p.timeout_ns);
+            tc_fence_after();
+            const uint64_t pd = base + s * desc_step, qd = pd + (kBP * kBK >> 4);
+            const uint32_t steps = p.ksteps - b * 4u;  // 1 to 3
+            if (one) {
+              mma_mx(d, pd, qd, idesc, sfp, sfq, accumulate);
+              if (steps > 1u) mma_mx(d, pd + 2u, qd + 2u, idesc, sfp, sfq, 1u);
+              if (steps > 2u) mma_mx(d, pd + 4u, qd + 4u, idesc, sfp, sfq, 1u);
+              commit_both(empty_base + s * 8u);
+            }
+            __syncwarp();
+            if (++s == p.stages) {
+              s = 0;
+              phase ^= 1u;
+            }
+          }
+          if (one) commit_both(smem_u32(&group_done[set]));
+          __syncwarp();
         }
-        if (ok) mma_commit(&acc_full[buf]);
+        if (one) commit_both(smem_u32(&acc_full[buf]));
+        ok = __all_sync(0xffffffffu, ok);
       }
       // Everything issued has completed before tensor memory is released.
-      mma_commit(&drained);
+      if (one) commit_both(smem_u32(&drained));
+      __syncwarp();
       uint32_t dummy = 0u;
-      mbar_wait(&drained, 0u, &dummy, p.err, p.timeout_ns);
+      if (lane == 0) mbar_wait(&drained, 0u, &dummy, p.err, p.timeout_ns);
     }
-  } else if (warp == 2) {
-    uint32_t group = 0;
-    bool ok = true;
-    for (uint32_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
-      const Unit t = unit_of(p, u);
-      for (uint32_t kb = t.kb0; kb < t.kb1; kb += 4u, ++group) {
-        uint32_t w[12];
-#pragma unroll
-        for (uint32_t i = 0; i < 12; ++i) {
-          const bool of_p = i < 4;
-          const uint32_t r = (of_p ? i : i - 4u) * 32u + lane;
-          const uint64_t row = of_p ? (uint64_t)t.p * kBP + r : (uint64_t)t.q * p.bn + r;
-          const bool in = of_p ? row < p.n : row < p.m && r < p.bn;
-          w[i] = in ? *reinterpret_cast<const uint32_t*>((of_p ? p.p_scales : p.q_scales) + row * p.scale_cols + kb) : 0u;
+  } else if (warp >= kScaleWarp && warp < kScaleWarp + 4u) {
+    // Row r of a tile has its word in lane r % 32, column r / 32, the same in
+    // every quadrant: this CTA's 128 rows of b, all BN rows of a.  Thread i
+    // fetches the words of row i of b and of rows i and i + 128 of a, a group
+    // ahead; shared memory hands them to all four warps.
+    const uint32_t quad = warp - kScaleWarp, i = threadIdx.x - kScaleWarp * 32u;
+    const uint32_t words_q = (p.bn + 31u) / 32u;
+    uint32_t u = unit0, group = 0, next[3] = {0u, 0u, 0u};
+    Unit t = {};
+    uint32_t kb = 0;
+    bool gave_up = false;
+    auto fetch = [&]() {  // the words of (t, kb)
+      const uint64_t pr = (uint64_t)(t.p * 2u + rank) * kBP + i, qr = (uint64_t)t.q * p.bn + i;
+      auto word = [&](const uint8_t* scales, uint64_t row) {
+        return __ldg(reinterpret_cast<const uint32_t*>(scales + row * p.scale_cols + kb));
+      };
+      next[0] = pr < p.n ? word(p.p_scales, pr) : 0u;
+      next[1] = i < p.bn && qr < p.m ? word(p.q_scales, qr) : 0u;
+      next[2] = i + 128u < p.bn && qr + 128u < p.m ? word(p.q_scales, qr + 128u) : 0u;
+    };
+    if (u < units) {
+      t = unit_of(p, u);
+      kb = t.kb0;
+      fetch();
+    }
+    while (u < units) {
+      uint32_t* words = scale_words[group & 1u];
+      words[i] = next[0];
+      words[kBP + i] = next[1];
+      words[kBP + 128u + i] = next[2];
+      // The four warps meet, and end together if one of them gave up waiting.
+      if (meet_any(gave_up)) break;
+      const uint32_t set = group % kSets, use = group / kSets;
+      kb += 4u;
+      if (kb >= t.kb1) {
+        u += ustep;
+        if (u < units) {
+          t = unit_of(p, u);
+          kb = t.kb0;
         }
-        const uint32_t sb = group % kScaleBufs;
-        const bool freed = lane != 0 || wait(&sf_empty[sb], ((group / kScaleBufs) & 1u) ^ 1u);
-        if (!__shfl_sync(0xffffffffu, freed ? 1u : 0u, 0)) {
-          ok = false;
-          break;
-        }
-        uint4* dst = reinterpret_cast<uint4*>(scales + sb * kScaleBytes) + lane;
-        dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        dst[32] = make_uint4(w[4], w[5], w[6], w[7]);
-        dst[64] = make_uint4(w[8], w[9], w[10], w[11]);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sf_full[sb]);
       }
+      if (u < units) fetch();
+      uint32_t w[12];
+#pragma unroll
+      for (uint32_t q = 0; q < 12; ++q) w[q] = words[q * 32u + lane];
+      // the set's last group has been read
+      const bool freed = lane != 0 || use == 0u || wait(&group_done[set], (use - 1u) & 1u);
+      gave_up = !__shfl_sync(0xffffffffu, freed ? 1u : 0u, 0);
+      if (!gave_up) {
+        tc_fence_after();
+        const uint32_t ta = tmem + kScaleCol + set * 16u + (quad << 21);
+        tmem_st_x4(ta, w);
+        tmem_st_x4(ta + 4u, w + 4);
+        if (words_q > 4u) tmem_st_x4(ta + 8u, w + 8);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_at(mapa_shared(&scale_full[set], 0));
+      }
+      ++group;
     }
-  } else if (warp >= 4) {
-    const uint32_t quad = warp - 4u;
+  } else if (warp >= kEpiWarp) {
+    // Two warps a lane quadrant, taking turns at sixteen columns.
+    const uint32_t quad = warp % 4u, turn = (warp - kEpiWarp) / 4u;
     uint32_t acc = 0;
-    for (uint32_t u = blockIdx.x; u < units; u += gridDim.x, ++acc) {
+    for (uint32_t u = unit0; u < units; u += ustep, ++acc) {
       const Unit t = unit_of(p, u);
       const uint32_t buf = acc & 1u;
       const bool full_ok = lane != 0 || wait(&acc_full[buf], (acc >> 1) & 1u);
       if (!__shfl_sync(0xffffffffu, full_ok ? 1u : 0u, 0)) break;
       tc_fence_after();
-      const uint64_t n = (uint64_t)t.p * kBP + quad * 32u + lane;
+      const uint64_t n = (uint64_t)(t.p * 2u + rank) * kBP + quad * 32u + lane;
       const uint64_t m0 = (uint64_t)t.q * p.bn;
-      const uint32_t rows = (uint32_t)min((uint64_t)p.bn, p.m - m0);
+      const uint32_t rows = n < p.n ? (uint32_t)min((uint64_t)p.bn, p.m - m0) : 0u;
       O* out;
       uint64_t stride;
       if constexpr (PARTS) {
@@ -285,26 +462,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         stride = p.out_stride;
       }
       const uint32_t ta = tmem + buf * kMaxBN + (quad << 21);  // lane quad * 32
-#pragma unroll 2
-      for (uint32_t c = 0; c < p.bn; c += 16u) {
-        uint32_t v[16];
-        tmem_ld_x16(ta + c, v);
+      uint32_t v[2][16];
+      uint32_t c = turn * 16u;
+      if (c < p.bn) tmem_ld_x16(ta + c, v[0]);
+      tmem_ld_wait();
+      while (c < p.bn) {  // the next columns load while these are stored
+        if (c + 32u < p.bn) tmem_ld_x16(ta + c + 32u, v[1]);
+        store16(out + c * stride, stride, v[0], rows > c ? rows - c : 0u);
         tmem_ld_wait();
-        if (n < p.n) {
-#pragma unroll
-          for (uint32_t i = 0; i < 16; ++i)
-            if (c + i < rows) out[(c + i) * stride] = from_f32<O>(__uint_as_float(v[i]));
-        }
+        c += 32u;
+        if (c >= p.bn) break;
+        if (c + 32u < p.bn) tmem_ld_x16(ta + c + 32u, v[0]);
+        store16(out + c * stride, stride, v[1], rows > c ? rows - c : 0u);
+        tmem_ld_wait();
+        c += 32u;
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+      if (lane == 0) arrive_at(mapa_shared(&acc_empty[buf], 0));
     }
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync();  // no arrival, copy or MMA of the peer is under way on this CTA's memory
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, 512);
+  if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
 // out = the parts' sum in order of K.
@@ -324,28 +506,29 @@ struct Plan {
   uint32_t bn, tiles_p, tiles_q, splits, split_groups;
 };
 
-// Rows of a a tile and splits of K by the estimated cycles of the busiest SM:
-// a block of K takes 2 BN cycles of the tensor core (not less than the 64 or
-// so that its stage's bytes take to arrive), a tile about 1000 + 4 BN beside
-// its MMAs, a split its parts' traffic and a second launch.
+// Rows of a a tile and splits of K by the estimated cycles of the busiest
+// pair: a block of K takes 2 BN cycles of the tensor cores (not less than the
+// 128 or so that its 16 KB of b alone take to arrive), a tile about 1000 + 4 BN
+// beside its MMAs, a split its parts' traffic and a second launch.
 inline Plan plan(uint64_t m, uint64_t n, uint64_t k, int sm_count) {
   Plan best = {};
   double best_cost = 0.0;
-  const uint32_t groups = (uint32_t)div_up(k, 512), tp = (uint32_t)div_up(n, kBP);
+  const uint32_t pairs = (uint32_t)sm_count / 2u;
+  const uint32_t groups = (uint32_t)div_up(k, 512), tp = (uint32_t)div_up(n, 2 * kBP);
   const uint64_t least = div_up(m, kMaxBN);
   for (uint64_t tq = least; tq <= least + 8 && tq <= div_up(m, 16); ++tq) {
     const uint32_t bn = (uint32_t)(div_up(div_up(m, tq), 16) * 16);
     if (div_up(m, bn) != tq) continue;
     // splitting pays only while whole tiles leave SMs without work
-    const uint32_t most = (uint64_t)tp * tq >= (uint64_t)sm_count ? 1u : 32u;
+    const uint32_t most = (uint64_t)tp * tq >= (uint64_t)pairs ? 1u : 32u;
     for (uint32_t want = 1; want <= groups && want <= most; ++want) {
       const uint32_t sg = (uint32_t)div_up(groups, want), splits = (uint32_t)div_up(groups, sg);
       if (splits != want) continue;
       const double units = (double)tp * (double)tq * splits;
-      if (splits > 1 && units > 2.0 * sm_count) break;
+      if (splits > 1 && units > 2.0 * pairs) break;
       const double blocks = sg * 4.0 < (double)div_up(k, 128) ? sg * 4.0 : (double)div_up(k, 128);
-      const double waves = (double)(uint64_t)((units + sm_count - 1) / sm_count);
-      double cost = waves * (blocks * (2.0 * bn > 64.0 ? 2.0 * bn : 64.0) + 1000.0 + 4.0 * bn);
+      const double waves = (double)(uint64_t)((units + pairs - 1) / pairs);
+      double cost = waves * (blocks * (2.0 * bn > 128.0 ? 2.0 * bn : 128.0) + 1000.0 + 4.0 * bn);
       if (splits > 1) cost += 5000.0 + 8.0 * splits * (double)m * (double)n / 3500.0;
       if (best.bn == 0 || cost < best_cost) {
         best = {bn, tp, (uint32_t)tq, splits, sg};
@@ -384,7 +567,7 @@ cudaError_t launch_matmul_fp8(const tessa_fp8_matmul_args& a, void* workspace, c
   const mm::Plan pl = mm::plan(a.m, a.n, a.k, c.sm_count);
   CUtensorMap pm, qm;
   if (make_code_tmap(&pm, a.b_codes, a.n, (uint32_t)a.k, mm::kBP) != 0 ||
-      make_code_tmap(&qm, a.a_codes, a.m, (uint32_t)a.k, pl.bn) != 0)
+      make_code_tmap(&qm, a.a_codes, a.m, (uint32_t)a.k, pl.bn / 2) != 0)
     return cudaErrorInvalidValue;
   mm::Params p = {};
   p.p_scales = a.b_scales;
@@ -399,17 +582,17 @@ cudaError_t launch_matmul_fp8(const tessa_fp8_matmul_args& a, void* workspace, c
   p.tiles_q = pl.tiles_q;
   p.splits = pl.splits;
   p.split_groups = pl.split_groups;
-  const uint32_t stage = (mm::kBP + pl.bn) * mm::kBK, fixed = 1024u + mm::kScaleBufs * mm::kScaleBytes + 1024u;
-  p.stages = (mm::kSmemLimit - fixed) / stage;
+  const uint32_t stage = (mm::kBP + pl.bn / 2) * mm::kBK;
+  p.stages = (mm::kSmemLimit - 5120u) / stage;  // beside the stages: alignment, barriers and scale words
   if (p.stages > mm::kMaxStages) p.stages = mm::kMaxStages;
   p.out = a.out;
   p.out_stride = a.out_stride;
   p.parts = static_cast<float*>(workspace);
   p.err = c.err;
   p.timeout_ns = c.timeout_ns;
-  const uint32_t smem = p.stages * stage + mm::kScaleBufs * mm::kScaleBytes + 1024u;
-  const uint64_t units = (uint64_t)pl.tiles_p * pl.tiles_q * pl.splits;
-  const uint32_t grid = (uint32_t)(units < (uint64_t)c.sm_count ? units : (uint64_t)c.sm_count);
+  const uint32_t smem = p.stages * stage + 1024u;
+  const uint64_t units = (uint64_t)pl.tiles_p * pl.tiles_q * pl.splits, pairs = (uint64_t)c.sm_count / 2;
+  const uint32_t grid = 2u * (uint32_t)(units < pairs ? units : pairs);
   if (pl.splits > 1) {
     cudaError_t e = mm::launch<float, true>(pm, qm, p, smem, grid, stream);
     if (e != cudaSuccess) return e;
