@@ -285,6 +285,7 @@ struct tessa_ctx {
   SubmitRing* ring = nullptr;       // subtree submissions (created on first use)
   uint32_t leaf_kernel = 1;         // 0: column-split kernel on CTA pairs where it applies, 1: one CTA per tile
   uint32_t* async_err = nullptr;    // pinned, mapped error word of the calls that do not wait (created on first use)
+  uint32_t* async_err_dev = nullptr;
 };
 
 namespace {
@@ -771,14 +772,19 @@ int tessa::async_begin(tessa_ctx* ctx, AsyncCtx* out) {
     void* p = nullptr;
     CUDA_TRY(cudaHostAlloc(&p, 64, cudaHostAllocMapped));
     memset(p, 0, 64);
+    void* d = nullptr;
+    if (cudaError_t e = cudaHostGetDevicePointer(&d, p, 0)) {
+      cudaFreeHost(p);
+      return fail(TESSA_ERR_CUDA, "cudaHostGetDevicePointer: %s", cudaGetErrorString(e));
+    }
     ctx->async_err = static_cast<uint32_t*>(p);
+    ctx->async_err_dev = static_cast<uint32_t*>(d);
   }
   TRY(take_async_error(ctx));
+  out->device = ctx->device;
   out->sm_count = ctx->sm_count;
   out->timeout_ns = ctx->timeout_ns;
-  void* d = nullptr;
-  CUDA_TRY(cudaHostGetDevicePointer(&d, ctx->async_err, 0));
-  out->err = static_cast<uint32_t*>(d);
+  out->err = ctx->async_err_dev;
   return TESSA_OK;
 }
 

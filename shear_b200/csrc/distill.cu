@@ -44,6 +44,7 @@ struct DistillPlan {
 };
 
 constexpr uint32_t kNoEntry = 0xffffffffu;
+constexpr uint32_t kMaxKeep = 200u << 10;  // the largest slice a CTA keeps, beside the longest list
 
 template <class T, int WARPS>
 __global__ void __launch_bounds__((WARPS + 1) * 32)
@@ -259,7 +260,8 @@ template <class T, int WARPS>
 cudaError_t launch_distill_as(const tessa_distill_args& a, const DistillPlan& plan, const AsyncCtx& c,
                               cudaStream_t stream) {
   const uint32_t smem = (a.k + 3u) / 4u * 64u + plan.keep_bytes;
-  cudaError_t e = cudaFuncSetAttribute(distill_kernel<T, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static SmemRaised raised;
+  cudaError_t e = raise_smem(distill_kernel<T, WARPS>, c.device, kMaxKeep + 64 * 256, raised);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((uint32_t)(a.rows * plan.cluster));
@@ -288,7 +290,7 @@ cudaError_t launch_distill(const tessa_distill_args& a, const AsyncCtx& c, cudaS
                                                              bytes / plan.cluster > 16384)))
     plan.cluster *= 2;
   const uint64_t slice = div_up(bytes, plan.cluster) + 16;
-  if (a.grad && slice <= (200u << 10)) plan.keep_bytes = (uint32_t)(div_up(slice, 16) * 16);
+  if (a.grad && slice <= kMaxKeep) plan.keep_bytes = (uint32_t)(div_up(slice, 16) * 16);
   return with_type(a.dtype, [&](auto t) {
     if (slice <= 32768 + 16) return launch_distill_as<decltype(t), 8>(a, plan, c, stream);
     return launch_distill_as<decltype(t), 16>(a, plan, c, stream);

@@ -437,10 +437,11 @@ cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspa
     s.bins = 1u << p.digit_bits;
     if (s.bins < 2) s.bins = 2;
     const uint32_t smem = kSortWarps * s.bins * 4u;
-    for (auto k : {sort_scatter_kernel<true>, sort_scatter_kernel<false>}) {
-      cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-      if (e != cudaSuccess) return e;
-    }
+    static SmemRaised raised[2];
+    constexpr int kMost = kSortWarps * (1 << kMaxDigitBits) * 4;
+    cudaError_t e = raise_smem(sort_scatter_kernel<true>, c.device, kMost, raised[0]);
+    if (e == cudaSuccess) e = raise_smem(sort_scatter_kernel<false>, c.device, kMost, raised[1]);
+    if (e != cudaSuccess) return e;
     for (uint32_t pass = 0; pass < p.passes; ++pass) {
       out = pass & 1u;
       s.keys = at(g.keys[out ^ 1u]);

@@ -7,18 +7,19 @@
 // sum over K never leaves the f32 accumulator in tensor memory: no pass over
 // the accumulator per block, as a free f32 scale would need.
 //
-// Persistent pairs of CTAs (two SMs) share a tile of 256 rows of b and BN rows
-// of a: each CTA holds 128 rows of b and half of a's in shared memory, and one
-// MMA (cta_group::2) reads both halves, so a stage brings 31 KB into an SM
-// where a CTA alone would need 47 KB for the same work.  Roles, concurrently:
+// Persistent pairs of CTAs (two SMs) share a tile of 256 rows of a and BN rows
+// of b: each CTA holds 128 rows of a and half of b's in shared memory, and one
+// MMA (cta_group::2) reads both halves, so a stage brings 30 KB into an SM
+// where a CTA alone would need 44 KB for the same work.  Roles, concurrently:
 //   warp 0      TMA: stages of 128 bytes of K
 //   warp 1      tensor memory; in the first CTA the pair's MMAs
 //   warps 4-7   scales: 32-bit words (four blocks of K) from global memory to
 //               the four lane quadrants of tensor memory
 //   warps 8-15  epilogue: accumulators to global memory
-// b's rows are the accumulator's lanes and a's rows its columns, so a warp
-// holds 32 consecutive n of one m and stores them straight to out, and a batch
-// of few rows makes a narrow MMA (BN from 16) instead of a mostly empty one.
+// A thread of the epilogue holds one row of out, so it packs neighbouring
+// columns into 16-byte pieces of a swizzled box that TMA stores: about one
+// instruction a column.  (With b's rows in the lanes, a warp stores 32 columns
+// of one row at a time, five instructions a column.)
 // Two accumulators: one is emptied while the next is summed.
 //
 // K may be split over units (few tiles, long K): each unit writes f32 parts to
@@ -31,18 +32,23 @@ namespace train {
 namespace mm {
 
 constexpr uint32_t kThreads = 512;
-constexpr uint32_t kBP = 128;             // rows of b a CTA (accumulator lanes)
-constexpr uint32_t kMaxBN = 224;          // rows of a a tile: two accumulators leave 64 of 512 columns to the scales
+constexpr uint32_t kBP = 128;             // rows of a a CTA (accumulator lanes)
+constexpr uint32_t kMaxBN = 224;          // rows of b a tile: two accumulators leave 64 of 512 columns to the scales
 constexpr uint32_t kBK = 128;             // bytes of K a stage
 constexpr uint32_t kScaleCol = 448;       // tensor memory columns of the scales
 constexpr uint32_t kSets = 4;             // sets of 16: the scale warps run up to three groups ahead
+constexpr uint32_t kRing = 6, kAhead = 4;  // groups of scale words in shared memory, and under way of them
 constexpr uint32_t kMaxStages = 10;
+constexpr uint32_t kBoxBytes = 2048;      // one TMA store of a warp: 32 rows of 64 bytes
+constexpr uint32_t kBoxes = 2;            // a warp of the epilogue
 constexpr uint32_t kSmemLimit = 227u * 1024u;
+constexpr uint32_t kStatic = 10u * 1024u;  // barriers and scale words, and a little
+constexpr uint64_t kGivenUpNs = 1000000ull;  // for what is still under way after a wait gave up
 constexpr uint32_t kScaleWarp = 4, kEpiWarp = 8;
 
 struct Params {
-  const uint8_t* p_scales;  // b's
-  const uint8_t* q_scales;  // a's
+  const uint8_t* p_scales;  // a's
+  const uint8_t* q_scales;  // b's
   uint64_t scale_cols;
   uint64_t m, n;
   uint32_t kblocks;         // blocks of 128
@@ -50,10 +56,13 @@ struct Params {
   uint32_t bn;
   uint32_t tiles_p, tiles_q;
   uint32_t splits, split_groups;  // groups of four blocks a split
+  uint32_t raster;          // tiles along b that go together
   uint32_t stages;
   void* out;
   uint64_t out_stride;
-  float* parts;             // splits x m x n, splits > 1
+  float* parts;             // splits x m x parts_stride, splits > 1
+  uint64_t parts_stride;    // n rounded up to 4
+  uint32_t tma_out;         // out's rows suit TMA (16-byte base and stride); parts' always do
   uint32_t* err;
   uint64_t timeout_ns;
 };
@@ -71,15 +80,6 @@ __device__ __forceinline__ void mma_mx(uint32_t d, uint64_t adesc, uint64_t bdes
       "setp.ne.b32 p, %6, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate));
-}
-
-__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
 }
 
 __device__ __forceinline__ void tmem_st_x4(uint32_t taddr, const uint32_t* r) {
@@ -142,6 +142,12 @@ __device__ __forceinline__ bool wait_at(uint32_t bar, uint32_t parity, volatile 
                                           abort_flag, err, timeout_ns);
 }
 
+// Four bytes to shared memory, asynchronously; zero where there is no such row.
+__device__ __forceinline__ void copy_word(uint32_t* dst, const void* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(there ? 4u : 0u)
+               : "memory");
+}
+
 // Barrier of the four scale warps; whether any thread said so.
 __device__ __forceinline__ bool meet_any(bool said) {
   uint32_t r;
@@ -156,22 +162,37 @@ __device__ __forceinline__ bool meet_any(bool said) {
   return r != 0u;
 }
 
+template <class O>
+__device__ __forceinline__ uint4 pack8(const uint32_t* v) {
+  Vec<O, 8> o;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o.v[i] = from_f32<O>(__uint_as_float(v[i]));
+  return *reinterpret_cast<const uint4*>(&o);
+}
+
+__device__ __forceinline__ void store_box(const CUtensorMap* map, uint32_t box, int32_t x, int32_t y, int32_t z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(box), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+
 struct Unit {
   uint32_t p, q;       // tile
   uint32_t kb0, kb1;   // blocks of K
   uint32_t split;
 };
 
-// Tiles in blocks of up to 16 along a: the tiles in flight at a time then
-// share few rows of b and of a in L2.
+// Tiles in blocks of `raster` along b, a's tiles one after the other within a
+// block: the tiles in flight write neighbouring pieces of the same rows of out,
+// and find the block's rows of b in L2.
 __device__ __forceinline__ Unit unit_of(const Params& p, uint32_t u) {
   Unit r;
   r.split = u % p.splits;
   const uint32_t t = u / p.splits;
-  constexpr uint32_t kGroup = 16;
-  const uint32_t block = t / (kGroup * p.tiles_p), in = t % (kGroup * p.tiles_p);
-  const uint32_t wide = min(kGroup, p.tiles_q - block * kGroup);
-  r.q = block * kGroup + in % wide;
+  const uint32_t block = t / (p.raster * p.tiles_p), in = t % (p.raster * p.tiles_p);
+  const uint32_t wide = min(p.raster, p.tiles_q - block * p.raster);
+  r.q = block * p.raster + in % wide;
   r.p = in / wide;
   r.kb0 = r.split * p.split_groups * 4u;
   r.kb1 = min(p.kblocks, r.kb0 + p.split_groups * 4u);
@@ -188,20 +209,25 @@ __device__ __forceinline__ void span_of(const Params& p, uint32_t u, uint32_t& k
   }
 }
 
-// Sixteen accumulator columns of the lane's row: out[i * stride], i < rows.
+// 128 bytes of a row (32 f32 or 64 16-bit columns) of the accumulator as eight
+// 16-byte pieces.
 template <class O>
-__device__ __forceinline__ void store16(O* out, uint64_t stride, const uint32_t (&v)[16], uint32_t rows) {
-  if (rows >= 16u) {
+__device__ __forceinline__ void load_row(uint32_t taddr, uint4 (&piece)[8]) {
+  uint32_t v[32];
+  if constexpr (sizeof(O) == 4) {
+    tmem_ld_32x32b_x32(taddr, v);
+    tmem_ld_wait();
 #pragma unroll
-    for (uint32_t i = 0; i < 16; ++i) {
-      *out = from_f32<O>(__uint_as_float(v[i]));
-      out += stride;
-    }
+    for (uint32_t j = 0; j < 8; ++j) piece[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
   } else {
+    uint32_t w[32];
+    tmem_ld_32x32b_x32(taddr, v);
+    tmem_ld_32x32b_x32(taddr + 32u, w);
+    tmem_ld_wait();
 #pragma unroll
-    for (uint32_t i = 0; i < 16; ++i) {
-      if (i < rows) *out = from_f32<O>(__uint_as_float(v[i]));
-      out += stride;
+    for (uint32_t j = 0; j < 4; ++j) {
+      piece[j] = pack8<O>(v + 8 * j);
+      piece[4 + j] = pack8<O>(w + 8 * j);
     }
   }
 }
@@ -209,14 +235,14 @@ __device__ __forceinline__ void store16(O* out, uint64_t stride, const uint32_t 
 template <class O, bool PARTS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fp8_matmul_kernel(const __grid_constant__ CUtensorMap pmap, const __grid_constant__ CUtensorMap qmap,
-                      const Params p) {
+                      const __grid_constant__ CUtensorMap omap, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023u) & ~(uintptr_t)1023u);
   // In the first CTA: full, scale_full and acc_empty count both CTAs' work.
   // The other barriers are signalled in both CTAs.
   __shared__ __align__(8) uint64_t full[kMaxStages], empty[kMaxStages], scale_full[kSets], group_done[kSets],
       acc_full[2], acc_empty[2], drained;
-  __shared__ uint32_t scale_words[2][kBP + 256];  // a group's words: b's rows, a's rows
+  __shared__ uint32_t scale_words[kRing][kBP + 256];  // a group's words: a's rows, b's rows
   __shared__ uint32_t tmem_slot, abort_word;
   volatile uint32_t* abort_flag = &abort_word;
   const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
@@ -287,16 +313,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       ok = __all_sync(0xffffffffu, ok);
     }
-    // The block may not end before its copies have landed.  The first CTA sees
-    // both CTAs' bytes; after a wait gave up somewhere the other, whose copies
-    // may lack their counterpart, leaves them ample time instead.
-    if (lane == 0 && rank == 0) {
+    // The block may not end before its copies have landed and before the MMAs
+    // that read them have signalled both CTAs: a signal that came later would
+    // find no barrier.  Each stage's last use says both.
+    if (lane == 0) {
       uint32_t dummy = 0u;
+      const uint64_t limit = ok ? p.timeout_ns : kGivenUpNs;
       for (uint32_t i = filled > p.stages ? filled - p.stages : 0u; i < filled; ++i)
-        mbar_wait(&full[i % p.stages], (i / p.stages) & 1u, &dummy, p.err, p.timeout_ns);
-    } else if (lane == 0 && !ok) {
-      const uint64_t t0 = global_timer_ns();
-      while (global_timer_ns() - t0 < 1000000ull) __nanosleep(1000);
+        mbar_wait(&empty[i % p.stages], (i / p.stages) & 1u, &dummy, p.err, limit);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -332,9 +356,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const uint32_t end = min(kb + 4u, kb1), full_end = min(end, whole);
           uint32_t idesc = idesc_mx(p.bn, 0), b = kb;
           for (; b < full_end; ++b, idesc += idesc_mx(0, 1) - idesc_mx(0, 0)) {
+            const uint64_t pd = base + s * desc_step, qd = pd + (kBP * kBK >> 4);
             ok &= wait_at(full_base + s * 8u, phase, abort_flag, p.err, p.timeout_ns);
             tc_fence_after();
-            const uint64_t pd = base + s * desc_step, qd = pd + (kBP * kBK >> 4);
             if (one) {
               mma_mx(d, pd, qd, idesc, sfp, sfq, accumulate);
               mma_mx(d, pd + 2u, qd + 2u, idesc, sfp, sfq, 1u);
@@ -350,10 +374,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
           }
           if (b < end) {
-            ok &= wait_at(full_base + s * 8u, phase, abort_flag, p.err, p.timeout_ns);
-            tc_fence_after();
             const uint64_t pd = base + s * desc_step, qd = pd + (kBP * kBK >> 4);
             const uint32_t steps = p.ksteps - b * 4u;  // 1 to 3
+            ok &= wait_at(full_base + s * 8u, phase, abort_flag, p.err, p.timeout_ns);
+            tc_fence_after();
             if (one) {
               mma_mx(d, pd, qd, idesc, sfp, sfq, accumulate);
               if (steps > 1u) mma_mx(d, pd + 2u, qd + 2u, idesc, sfp, sfq, 1u);
@@ -380,49 +404,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
   } else if (warp >= kScaleWarp && warp < kScaleWarp + 4u) {
     // Row r of a tile has its word in lane r % 32, column r / 32, the same in
-    // every quadrant: this CTA's 128 rows of b, all BN rows of a.  Thread i
-    // fetches the words of row i of b and of rows i and i + 128 of a, a group
-    // ahead; shared memory hands them to all four warps.
+    // every quadrant: this CTA's 128 rows of a, all BN rows of b.  Thread i
+    // fetches the words of row i of a and of rows i and i + 128 of b into a
+    // ring in shared memory, kAhead groups before they are used (a group may
+    // be a whole tile, shorter than a load from HBM), and all four warps read
+    // them there.
     const uint32_t quad = warp - kScaleWarp, i = threadIdx.x - kScaleWarp * 32u;
     const uint32_t words_q = (p.bn + 31u) / 32u;
-    uint32_t u = unit0, group = 0, next[3] = {0u, 0u, 0u};
-    Unit t = {};
-    uint32_t kb = 0;
-    bool gave_up = false;
-    auto fetch = [&]() {  // the words of (t, kb)
+    uint32_t u = unit0, kb = 0, kb1 = 0, fetched = 0;  // the next group to fetch
+    const uint8_t *src_p = nullptr, *src_q = nullptr, *src_r = nullptr;
+    bool has_p = false, has_q = false, has_r = false;
+    auto open_unit = [&]() {
+      if (u >= units) return;
+      const Unit t = unit_of(p, u);
       const uint64_t pr = (uint64_t)(t.p * 2u + rank) * kBP + i, qr = (uint64_t)t.q * p.bn + i;
-      auto word = [&](const uint8_t* scales, uint64_t row) {
-        return __ldg(reinterpret_cast<const uint32_t*>(scales + row * p.scale_cols + kb));
-      };
-      next[0] = pr < p.n ? word(p.p_scales, pr) : 0u;
-      next[1] = i < p.bn && qr < p.m ? word(p.q_scales, qr) : 0u;
-      next[2] = i + 128u < p.bn && qr + 128u < p.m ? word(p.q_scales, qr + 128u) : 0u;
-    };
-    if (u < units) {
-      t = unit_of(p, u);
       kb = t.kb0;
-      fetch();
-    }
-    while (u < units) {
-      uint32_t* words = scale_words[group & 1u];
-      words[i] = next[0];
-      words[kBP + i] = next[1];
-      words[kBP + 128u + i] = next[2];
-      // The four warps meet, and end together if one of them gave up waiting.
-      if (meet_any(gave_up)) break;
-      const uint32_t set = group % kSets, use = group / kSets;
-      kb += 4u;
-      if (kb >= t.kb1) {
-        u += ustep;
-        if (u < units) {
-          t = unit_of(p, u);
-          kb = t.kb0;
+      kb1 = t.kb1;
+      has_p = pr < p.m;
+      has_q = i < p.bn && qr < p.n;
+      has_r = i + 128u < p.bn && qr + 128u < p.n;
+      src_p = p.p_scales + (has_p ? pr : 0u) * p.scale_cols;
+      src_q = p.q_scales + (has_q ? qr : 0u) * p.scale_cols;
+      src_r = p.q_scales + (has_r ? qr + 128u : 0u) * p.scale_cols;
+    };
+    auto fetch = [&]() {
+      if (u < units) {
+        uint32_t* words = scale_words[fetched % kRing];
+        copy_word(words + i, src_p + kb, has_p);
+        copy_word(words + kBP + i, src_q + kb, has_q);
+        copy_word(words + kBP + 128u + i, src_r + kb, has_r);
+        ++fetched;
+        kb += 4u;
+        if (kb >= kb1) {
+          u += ustep;
+          open_unit();
         }
       }
-      if (u < units) fetch();
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    open_unit();
+    for (uint32_t g = 0; g < kAhead; ++g) fetch();
+    bool gave_up = false;
+    uint32_t done = 0;  // groups handed to the MMAs
+    for (uint32_t group = 0; group < fetched; ++group) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+      // The four warps meet, and end together if one of them gave up waiting.
+      if (meet_any(gave_up)) break;
+      const uint32_t* words = scale_words[group % kRing];
       uint32_t w[12];
 #pragma unroll
       for (uint32_t q = 0; q < 12; ++q) w[q] = words[q * 32u + lane];
+      fetch();  // into the place of a group that all four have read (they have met since)
+      const uint32_t set = group % kSets, use = group / kSets;
       // the set's last group has been read
       const bool freed = lane != 0 || use == 0u || wait(&group_done[set], (use - 1u) & 1u);
       gave_up = !__shfl_sync(0xffffffffu, freed ? 1u : 0u, 0);
@@ -436,12 +469,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) arrive_at(mapa_shared(&scale_full[set], 0));
+        ++done;
       }
-      ++group;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    // The last groups' signals, too, come while this CTA is there.
+    if (quad == 0 && lane == 0) {
+      uint32_t dummy = 0u;
+      const uint64_t limit = *abort_flag ? kGivenUpNs : p.timeout_ns;
+      for (uint32_t g = done > kSets ? done - kSets : 0u; g < done; ++g)
+        mbar_wait(&group_done[g % kSets], (g / kSets) & 1u, &dummy, p.err, limit);
+    }
+    __syncwarp();
   } else if (warp >= kEpiWarp) {
-    // Two warps a lane quadrant, taking turns at sixteen columns.
+    // Two warps a lane quadrant take turns at 128 bytes of its rows.
     const uint32_t quad = warp % 4u, turn = (warp - kEpiWarp) / 4u;
+    uint8_t* boxes = smem + p.stages * stage_bytes + (warp - kEpiWarp) * kBoxes * kBoxBytes;
     uint32_t acc = 0;
     for (uint32_t u = unit0; u < units; u += ustep, ++acc) {
       const Unit t = unit_of(p, u);
@@ -449,38 +492,70 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const bool full_ok = lane != 0 || wait(&acc_full[buf], (acc >> 1) & 1u);
       if (!__shfl_sync(0xffffffffu, full_ok ? 1u : 0u, 0)) break;
       tc_fence_after();
-      const uint64_t n = (uint64_t)(t.p * 2u + rank) * kBP + quad * 32u + lane;
-      const uint64_t m0 = (uint64_t)t.q * p.bn;
-      const uint32_t rows = n < p.n ? (uint32_t)min((uint64_t)p.bn, p.m - m0) : 0u;
+      constexpr uint32_t kCols = 64u / sizeof(O);  // of a box, two boxes a turn; BN is a multiple of 32
+      const uint64_t m0 = (uint64_t)(t.p * 2u + rank) * kBP + quad * 32u, n0 = (uint64_t)t.q * p.bn;
+      const uint32_t cols = m0 < p.m ? (uint32_t)min((uint64_t)p.bn, p.n - n0) : 0u;
+      const uint32_t rows = m0 < p.m ? (uint32_t)min((uint64_t)32u, p.m - m0) : 0u;
+      const uint32_t ta = tmem + buf * kMaxBN + (quad << 21);  // lane quad * 32
       O* out;
       uint64_t stride;
       if constexpr (PARTS) {
-        out = reinterpret_cast<O*>(p.parts) + ((uint64_t)t.split * p.m + m0) * p.n + n;
-        stride = p.n;
+        out = reinterpret_cast<O*>(p.parts) + ((uint64_t)t.split * p.m + m0) * p.parts_stride + n0;
+        stride = p.parts_stride;
       } else {
-        out = static_cast<O*>(p.out) + m0 * p.out_stride + n;
+        out = static_cast<O*>(p.out) + m0 * p.out_stride + n0;
         stride = p.out_stride;
       }
-      const uint32_t ta = tmem + buf * kMaxBN + (quad << 21);  // lane quad * 32
-      uint32_t v[2][16];
-      uint32_t c = turn * 16u;
-      if (c < p.bn) tmem_ld_x16(ta + c, v[0]);
-      tmem_ld_wait();
-      while (c < p.bn) {  // the next columns load while these are stored
-        if (c + 32u < p.bn) tmem_ld_x16(ta + c + 32u, v[1]);
-        store16(out + c * stride, stride, v[0], rows > c ? rows - c : 0u);
-        tmem_ld_wait();
-        c += 32u;
-        if (c >= p.bn) break;
-        if (c + 32u < p.bn) tmem_ld_x16(ta + c + 32u, v[0]);
-        store16(out + c * stride, stride, v[1], rows > c ? rows - c : 0u);
-        tmem_ld_wait();
-        c += 32u;
+      for (uint32_t c = turn * 2u * kCols; c < cols; c += 4u * kCols) {
+        uint4 piece[8];
+        load_row<O>(ta + c, piece);  // may read past BN into other columns of the allocation
+        const uint32_t width = min(2u * kCols, cols - c);
+        if ((PARTS || p.tma_out) && rows <= 4u && width == 2u * kCols) {
+          // few rows: sixteen bytes at a time, sooner done than a store by TMA
+          if (lane < rows) {
+            uint4* dst = reinterpret_cast<uint4*>(out + lane * stride + c);
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j) dst[j] = piece[j];
+          }
+          __syncwarp();  // the next load is the whole warp's
+          continue;
+        }
+        // the last stores out of the boxes have read them
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j)
+          *reinterpret_cast<uint4*>(boxes + j / 4u * kBoxBytes + lane * 64u + ((j ^ (lane >> 1)) & 3u) * 16u) = piece[j];
+        if (PARTS || p.tma_out) {  // out's right and lower edges TMA cuts
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            store_box(&omap, smem_u32(boxes), (int32_t)(n0 + c), (int32_t)m0, (int32_t)t.split);
+            if (width > kCols)
+              store_box(&omap, smem_u32(boxes) + kBoxBytes, (int32_t)(n0 + c + kCols), (int32_t)m0, (int32_t)t.split);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        } else {
+          __syncwarp();
+          constexpr uint32_t kPiece = 16u / sizeof(O);  // columns of a piece
+          for (uint32_t k = lane; k < width; k += 32u) {
+            const uint8_t* box = boxes + k / kCols * kBoxBytes;
+            const uint32_t j = k % kCols / kPiece;
+            O* dst = out + c + k;
+#pragma unroll 8
+            for (uint32_t r = 0; r < rows; ++r, dst += stride)
+              *dst = reinterpret_cast<const O*>(box + r * 64u + ((j ^ (r >> 1)) & 3u) * 16u)[k % kPiece];
+          }
+          __syncwarp();
+        }
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_at(mapa_shared(&acc_empty[buf], 0));
     }
+    // the boxes may not go before the stores have read them
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
@@ -489,16 +564,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
-// out = the parts' sum in order of K.
+// out = the parts' sum in order of K; a row of blocks to a row of out, four
+// columns a thread.
 template <class O>
-__global__ void __launch_bounds__(256) add_parts_kernel(const float* parts, uint32_t splits, uint64_t m, uint64_t n,
-                                                        O* out, uint64_t out_stride) {
-  const uint64_t total = m * n, step = (uint64_t)gridDim.x * 256u;
-  for (uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x; i < total; i += step) {
-    float s = parts[i];
+__global__ void __launch_bounds__(128) add_parts_kernel(const float* parts, uint64_t parts_stride, uint32_t splits,
+                                                        uint64_t m, uint64_t n, O* out, uint64_t out_stride, bool vec) {
+  const uint64_t n0 = ((uint64_t)blockIdx.x * 128u + threadIdx.x) * 4u, total = m * parts_stride;
+  if (n0 >= n) return;
+  for (uint64_t r = blockIdx.y; r < m; r += gridDim.y) {
+    const float* src = parts + r * parts_stride + n0;
+    O* dst = out + r * out_stride + n0;
+    float4 s = __ldcs(reinterpret_cast<const float4*>(src));
 #pragma unroll 4
-    for (uint32_t k = 1; k < splits; ++k) s += parts[(uint64_t)k * total + i];
-    out[i / n * out_stride + i % n] = from_f32<O>(s);
+    for (uint32_t k = 1; k < splits; ++k) {
+      const float4 v = __ldcs(reinterpret_cast<const float4*>(src + k * total));
+      s.x += v.x;
+      s.y += v.y;
+      s.z += v.z;
+      s.w += v.w;
+    }
+    Vec<O, 4> o;
+    o.v[0] = from_f32<O>(s.x);
+    o.v[1] = from_f32<O>(s.y);
+    o.v[2] = from_f32<O>(s.z);
+    o.v[3] = from_f32<O>(s.w);
+    if (vec) {  // rows of out aligned to four elements, n a multiple of 4
+      *reinterpret_cast<Vec<O, 4>*>(dst) = o;
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i)
+        if (n0 + i < n) dst[i] = o.v[i];
+    }
   }
 }
 
@@ -506,29 +602,32 @@ struct Plan {
   uint32_t bn, tiles_p, tiles_q, splits, split_groups;
 };
 
-// Rows of a a tile and splits of K by the estimated cycles of the busiest
-// pair: a block of K takes 2 BN cycles of the tensor cores (not less than the
-// 128 or so that its 16 KB of b alone take to arrive), a tile about 1000 + 4 BN
-// beside its MMAs, a split its parts' traffic and a second launch.
+// Rows of b a tile and splits of K by the estimated cycles of the busiest
+// pair: a block of K takes 2 BN cycles of the tensor cores (156 at least: the
+// four MMAs' issue), a tile about 1500 beside its MMAs, a split its parts'
+// traffic and a second launch.
 inline Plan plan(uint64_t m, uint64_t n, uint64_t k, int sm_count) {
   Plan best = {};
   double best_cost = 0.0;
   const uint32_t pairs = (uint32_t)sm_count / 2u;
-  const uint32_t groups = (uint32_t)div_up(k, 512), tp = (uint32_t)div_up(n, 2 * kBP);
-  const uint64_t least = div_up(m, kMaxBN);
-  for (uint64_t tq = least; tq <= least + 8 && tq <= div_up(m, 16); ++tq) {
-    const uint32_t bn = (uint32_t)(div_up(div_up(m, tq), 16) * 16);
-    if (div_up(m, bn) != tq) continue;
+  const uint32_t groups = (uint32_t)div_up(k, 512), tp = (uint32_t)div_up(m, 2 * kBP);
+  const uint64_t least = div_up(n, kMaxBN);
+  // tile counts that fill whole rounds of the SM pairs, and the fewest
+  const uint64_t wave = pairs / tp ? pairs / tp : 1;
+  for (uint64_t i = 0; i < 12; ++i) {
+    const uint64_t tq = i < 8 ? least + i : div_up(least, wave) * wave + (i - 8) * wave;
+    if (tq > div_up(n, 32)) continue;
+    const uint32_t bn = (uint32_t)(div_up(div_up(n, tq), 32) * 32);
+    if (div_up(n, bn) != tq) continue;
     // splitting pays only while whole tiles leave SMs without work
     const uint32_t most = (uint64_t)tp * tq >= (uint64_t)pairs ? 1u : 32u;
     for (uint32_t want = 1; want <= groups && want <= most; ++want) {
       const uint32_t sg = (uint32_t)div_up(groups, want), splits = (uint32_t)div_up(groups, sg);
       if (splits != want) continue;
-      const double units = (double)tp * (double)tq * splits;
-      if (splits > 1 && units > 2.0 * pairs) break;
+      const uint64_t units = (uint64_t)tp * tq * splits;
+      if (splits > 1 && units > 2 * pairs) break;
       const double blocks = sg * 4.0 < (double)div_up(k, 128) ? sg * 4.0 : (double)div_up(k, 128);
-      const double waves = (double)(uint64_t)((units + pairs - 1) / pairs);
-      double cost = waves * (blocks * (2.0 * bn > 128.0 ? 2.0 * bn : 128.0) + 1000.0 + 4.0 * bn);
+      double cost = (double)div_up(units, pairs) * (blocks * (2.0 * bn > 156.0 ? 2.0 * bn : 156.0) + 1500.0);
       if (splits > 1) cost += 5000.0 + 8.0 * splits * (double)m * (double)n / 3500.0;
       if (best.bn == 0 || cost < best_cost) {
         best = {bn, tp, (uint32_t)tq, splits, sg};
@@ -539,13 +638,33 @@ inline Plan plan(uint64_t m, uint64_t n, uint64_t k, int sm_count) {
   return best;
 }
 
+// The plan of the calling thread's last few shapes (the search takes longer
+// than a launch).
+inline Plan plan_of(uint64_t m, uint64_t n, uint64_t k, int sm_count) {
+  struct Entry {
+    uint64_t m = 0, n = 0, k = 0;
+    int sms = 0;
+    Plan plan;
+  };
+  thread_local Entry kept[16];
+  Entry& e = kept[(m * 31 + n * 7 + k / 16) % 16];
+  if (e.m != m || e.n != n || e.k != k || e.sms != sm_count) {
+    e.plan = plan(m, n, k, sm_count);
+    e.m = m;
+    e.n = n;
+    e.k = k;
+    e.sms = sm_count;
+  }
+  return e.plan;
+}
+
 template <class O, bool PARTS>
-cudaError_t launch(const CUtensorMap& pm, const CUtensorMap& qm, const Params& p, uint32_t smem, uint32_t grid,
-                   cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(fp8_matmul_kernel<O, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)smem);
+cudaError_t launch(const CUtensorMap& pm, const CUtensorMap& qm, const CUtensorMap& om, const Params& p, int device, uint32_t smem,
+                   uint32_t grid, cudaStream_t stream) {
+  static SmemRaised raised;
+  cudaError_t e = raise_smem(fp8_matmul_kernel<O, PARTS>, device, (int)(kSmemLimit - kStatic), raised);
   if (e != cudaSuccess) return e;
-  fp8_matmul_kernel<O, PARTS><<<grid, kThreads, smem, stream>>>(pm, qm, p);
+  fp8_matmul_kernel<O, PARTS><<<grid, kThreads, smem, stream>>>(pm, qm, om, p);
   return cudaGetLastError();
 }
 
@@ -554,8 +673,8 @@ cudaError_t launch(const CUtensorMap& pm, const CUtensorMap& qm, const Params& p
 
 uint64_t fp8_matmul_workspace(uint64_t m, uint64_t n, uint64_t k, int sm_count) {
   if (m == 0 || n == 0 || k == 0) return 0;
-  const train::mm::Plan pl = train::mm::plan(m, n, k, sm_count);
-  return pl.splits > 1 ? (uint64_t)pl.splits * m * n * 4 : 0;
+  const train::mm::Plan pl = train::mm::plan_of(m, n, k, sm_count);
+  return pl.splits > 1 ? (uint64_t)pl.splits * m * train::div_up(n, 4) * 16 : 0;
 }
 
 cudaError_t launch_matmul_fp8(const tessa_fp8_matmul_args& a, void* workspace, const AsyncCtx& c,
@@ -564,14 +683,14 @@ cudaError_t launch_matmul_fp8(const tessa_fp8_matmul_args& a, void* workspace, c
   if (a.k == 0)
     return cudaMemset2DAsync(a.out, (a.m > 1 ? a.out_stride : a.n) * type_bytes(a.out_dtype), 0,
                              a.n * type_bytes(a.out_dtype), a.m, stream);
-  const mm::Plan pl = mm::plan(a.m, a.n, a.k, c.sm_count);
-  CUtensorMap pm, qm;
-  if (make_code_tmap(&pm, a.b_codes, a.n, (uint32_t)a.k, mm::kBP) != 0 ||
-      make_code_tmap(&qm, a.a_codes, a.m, (uint32_t)a.k, pl.bn / 2) != 0)
+  const mm::Plan pl = mm::plan_of(a.m, a.n, a.k, c.sm_count);
+  CUtensorMap pm, qm, om = {};
+  if (make_code_tmap(&pm, a.a_codes, a.m, (uint32_t)a.k, mm::kBP) != 0 ||
+      make_code_tmap(&qm, a.b_codes, a.n, (uint32_t)a.k, pl.bn / 2) != 0)
     return cudaErrorInvalidValue;
   mm::Params p = {};
-  p.p_scales = a.b_scales;
-  p.q_scales = a.a_scales;
+  p.p_scales = a.a_scales;
+  p.q_scales = a.b_scales;
   p.scale_cols = div_up(a.k, 512) * 4;
   p.m = a.m;
   p.n = a.n;
@@ -582,30 +701,45 @@ cudaError_t launch_matmul_fp8(const tessa_fp8_matmul_args& a, void* workspace, c
   p.tiles_q = pl.tiles_q;
   p.splits = pl.splits;
   p.split_groups = pl.split_groups;
+  // one tile an SM pair, as far as 32 MB of b go
+  const uint64_t fit = (32ull << 20) / (a.k * pl.bn), pairs = (uint64_t)c.sm_count / 2;
+  p.raster = (uint32_t)(fit > pairs ? pairs : fit < 8 ? 8 : fit);
   const uint32_t stage = (mm::kBP + pl.bn / 2) * mm::kBK;
-  p.stages = (mm::kSmemLimit - 5120u) / stage;  // beside the stages: alignment, barriers and scale words
+  const uint32_t boxes = 8u * mm::kBoxes * mm::kBoxBytes;
+  p.stages = (mm::kSmemLimit - mm::kStatic - 1024u - boxes) / stage;
   if (p.stages > mm::kMaxStages) p.stages = mm::kMaxStages;
   p.out = a.out;
   p.out_stride = a.out_stride;
   p.parts = static_cast<float*>(workspace);
+  p.parts_stride = div_up(a.n, 4) * 4;
+  if (pl.splits > 1) {
+    if (make_store_tmap(&om, p.parts, TESSA_F32, a.m, a.n, p.parts_stride, pl.splits) != 0)
+      return cudaErrorInvalidValue;
+  } else {
+    const uint32_t ob = type_bytes(a.out_dtype);
+    const uint64_t stride = a.m > 1 ? a.out_stride : div_up(a.n, 8) * 8;
+    p.tma_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && stride * ob % 16 == 0 &&
+                make_store_tmap(&om, a.out, a.out_dtype, a.m, a.n, stride, 1) == 0;
+  }
   p.err = c.err;
   p.timeout_ns = c.timeout_ns;
-  const uint32_t smem = p.stages * stage + 1024u;
-  const uint64_t units = (uint64_t)pl.tiles_p * pl.tiles_q * pl.splits, pairs = (uint64_t)c.sm_count / 2;
+  const uint32_t smem = p.stages * stage + boxes + 1024u;
+  const uint64_t units = (uint64_t)pl.tiles_p * pl.tiles_q * pl.splits;
   const uint32_t grid = 2u * (uint32_t)(units < pairs ? units : pairs);
   if (pl.splits > 1) {
-    cudaError_t e = mm::launch<float, true>(pm, qm, p, smem, grid, stream);
+    cudaError_t e = mm::launch<float, true>(pm, qm, om, p, c.device, smem, grid, stream);
     if (e != cudaSuccess) return e;
-    const uint64_t want = div_up(a.m * a.n, 256), most = (uint64_t)c.sm_count * 16;
+    const bool vec = vector_elems(a.out, a.m, a.n, a.out_stride, type_bytes(a.out_dtype), 4) == 4;
+    const dim3 blocks((uint32_t)div_up(a.n, 512), (uint32_t)(a.m < 32768 ? a.m : 32768));
     return with_type(a.out_dtype, [&](auto o) {
       using O = decltype(o);
-      mm::add_parts_kernel<O><<<(uint32_t)(want < most ? want : most), 256, 0, stream>>>(
-          p.parts, pl.splits, a.m, a.n, static_cast<O*>(a.out), a.out_stride);
+      mm::add_parts_kernel<O><<<blocks, 128, 0, stream>>>(p.parts, p.parts_stride, pl.splits, a.m, a.n,
+                                                          static_cast<O*>(a.out), a.out_stride, vec);
       return cudaGetLastError();
     });
   }
   return with_type(a.out_dtype,
-                   [&](auto o) { return mm::launch<decltype(o), false>(pm, qm, p, smem, grid, stream); });
+                   [&](auto o) { return mm::launch<decltype(o), false>(pm, qm, om, p, c.device, smem, grid, stream); });
 }
 
 }  // namespace tessa

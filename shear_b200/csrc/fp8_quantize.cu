@@ -162,11 +162,11 @@ __global__ void __launch_bounds__(256) quantize_tiles_kernel(const tessa_fp8_qua
 }
 
 template <class T, int VE, bool ROWS>
-cudaError_t launch_tiles(const tessa_fp8_quantize_args& a, uint32_t cc, uint32_t sc, uint32_t cr, uint32_t sr,
+cudaError_t launch_tiles(const tessa_fp8_quantize_args& a, int device, uint32_t cc, uint32_t sc, uint32_t cr, uint32_t sr,
                          cudaStream_t stream) {
   const uint32_t smem = 128u * 128u * sizeof(T);
-  cudaError_t e = cudaFuncSetAttribute(quantize_tiles_kernel<T, VE, ROWS>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static SmemRaised raised;
+  cudaError_t e = raise_smem(quantize_tiles_kernel<T, VE, ROWS>, device, (int)smem, raised);
   if (e != cudaSuccess) return e;
   const uint32_t ct = (uint32_t)div_up(a.cols, 128), rt = (uint32_t)div_up(a.rows, 128);
   quantize_tiles_kernel<T, VE, ROWS><<<ct * rt, 256, smem, stream>>>(a, ct, rt, cc, sc, cr, sr);
@@ -184,10 +184,10 @@ cudaError_t launch_quantize_fp8(const tessa_fp8_quantize_args& a, const AsyncCtx
     using T = decltype(t);
     if (a.codes_t) {
       if (a.codes)
-        return vec ? launch_tiles<T, 4, true>(a, code_cols, scale_cols, code_rows, scale_rows, stream)
-                   : launch_tiles<T, 1, true>(a, code_cols, scale_cols, code_rows, scale_rows, stream);
-      return vec ? launch_tiles<T, 4, false>(a, code_cols, scale_cols, code_rows, scale_rows, stream)
-                 : launch_tiles<T, 1, false>(a, code_cols, scale_cols, code_rows, scale_rows, stream);
+        return vec ? launch_tiles<T, 4, true>(a, c.device, code_cols, scale_cols, code_rows, scale_rows, stream)
+                   : launch_tiles<T, 1, true>(a, c.device, code_cols, scale_cols, code_rows, scale_rows, stream);
+      return vec ? launch_tiles<T, 4, false>(a, c.device, code_cols, scale_cols, code_rows, scale_rows, stream)
+                 : launch_tiles<T, 1, false>(a, c.device, code_cols, scale_cols, code_rows, scale_rows, stream);
     }
     const uint32_t blocks = (uint32_t)div_up(a.cols, 128);
     const uint64_t want = div_up(a.rows * scale_cols, 8), most = (uint64_t)c.sm_count * 32;

@@ -240,6 +240,7 @@ size_t reservoir_scratch_bytes(uint64_t edges, uint64_t num_points);
 // binds its device and reports what an earlier call's kernel left in the
 // mapped error word `err`.
 struct AsyncCtx {
+  int device;
   int sm_count;
   uint64_t timeout_ns;
   uint32_t* err;
@@ -261,6 +262,12 @@ cudaError_t launch_distill(const tessa_distill_args& a, const AsyncCtx& c, cudaS
 // 2-D uint8 tensor map (leaf_sq8.cu): rows x row_bytes, box of 128 bytes x
 // box_rows, 128-byte swizzle, zero fill.
 int make_code_tmap(CUtensorMap* map, const void* base, uint64_t rows, uint32_t row_bytes, uint32_t box_rows);
+
+// Map for stores of 2 KB boxes, 64 bytes wide and 32 rows high, 64-byte
+// swizzle: depth slices of rows x cols elements (type code `dtype`, row stride
+// in elements, slices rows * stride apart).
+int make_store_tmap(CUtensorMap* map, const void* base, uint32_t dtype, uint64_t rows, uint64_t cols, uint64_t stride,
+                    uint64_t depth);
 
 // Records `code` and `message` as the calling thread's last error (returned by
 // tessa_last_error_message); returns `code`.

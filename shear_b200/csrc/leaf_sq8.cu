@@ -807,6 +807,23 @@ int make_code_tmap(CUtensorMap* map, const void* base, uint64_t rows, uint32_t r
   return r == CUDA_SUCCESS ? 0 : -2;
 }
 
+int make_store_tmap(CUtensorMap* map, const void* base, uint32_t dtype, uint64_t rows, uint64_t cols, uint64_t stride,
+                    uint64_t depth) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return -1;
+  const uint32_t bytes = dtype == TESSA_F32 ? 4u : 2u;
+  cuuint64_t dims[3] = {cols, rows, depth};
+  cuuint64_t strides[2] = {stride * bytes, rows * stride * bytes};
+  cuuint32_t box[3] = {64 / bytes, 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUtensorMapDataType type = dtype == TESSA_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                             : dtype == TESSA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUresult r = enc(map, type, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -2;
+}
+
 // Shared-memory plan for a launch: B-operand stages and log entries per row.
 // Prefers >= 3 stages with a log of k + 24 entries; falls back to 2 stages
 // with at least k + 8.  Returns false if neither fits.

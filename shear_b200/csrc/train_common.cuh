@@ -1,6 +1,7 @@
 // Element types, aligned vectors and dispatch shared by the kernels that train
 // a table of vectors (embedding.cu, fp8_quantize.cu, fp8_matmul.cu, distill.cu).
 #pragma once
+#include <atomic>
 #include <type_traits>
 
 #include <cuda_bf16.h>
@@ -48,6 +49,20 @@ cudaError_t with_type(uint32_t dtype, F f) {
     case TESSA_BF16: return f(__nv_bfloat16());
     default: return f(__half());
   }
+}
+
+// Raises a kernel's dynamic shared memory limit to the device's, once a device
+// (`done`: a static of the caller, one a kernel).
+struct SmemRaised {
+  std::atomic<uint64_t> devices{0};
+};
+template <class K>
+cudaError_t raise_smem(K* kernel, int device, int most, SmemRaised& done) {
+  const uint64_t bit = 1ull << (device & 63);
+  if (done.devices.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (e == cudaSuccess) done.devices.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 inline uint32_t type_bytes(uint32_t dtype) { return dtype == TESSA_F32 ? 4u : 2u; }

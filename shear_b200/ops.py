@@ -797,53 +797,77 @@ def reduce_grouped(pieces, num_points: int, l_max: int, ctx: Context | None = No
 # error (an id outside the table) is reported by the next of them on the
 # context or by async_status(); ids of -1 are padding.  uint32 id tensors do
 # not occur here: ids are int32 or int64.
+#
+# A small batch takes the GPU a few microseconds, so the checks are written to
+# cost little: torch is imported once, devices are compared as indices, and
+# the current stream is taken as the raw handle.
 
-_DTYPES = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}
+_torch = None
+_DTYPES: dict = {}
+_ID_BITS: dict = {}
+
+
+def _lazy_torch():
+    global _torch
+    if _torch is None:
+        import torch
+
+        _DTYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+        _ID_BITS.update({torch.int32: 32, torch.int64: 64})
+        _torch = torch
+    return _torch
+
+
+def _stream(dev: int):
+    """The device's current stream as the C ABI takes it."""
+    return _torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _dtype_code(name: str, dtype) -> int:
-    code = _DTYPES.get(str(dtype))
+    code = _DTYPES.get(dtype)
     if code is None:
         raise ValueError(f"{name} must be float32, bfloat16 or float16, not {dtype}")
     return code
 
 
-def _matrix(name: str, t, device=None):
-    """Checks a 2-D device matrix with unit column stride; returns its row stride."""
+def _matrix(name: str, t, dev=None):
+    """Checks a 2-D device matrix with unit column stride.
+
+    Returns (rows, columns, row stride, type code); dev: the device index it must be on."""
     if t.dim() != 2 or not t.is_cuda:
         raise ValueError(f"{name} must be a 2-D CUDA tensor")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    if dev is not None and t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{dev}")
     rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
+    step, one = t.stride()
+    if one != 1 and cols > 1:
         raise ValueError(f"{name} must have contiguous rows (column stride 1)")
-    stride = t.stride(0) if rows > 1 else max(cols, t.stride(0))
-    if rows > 1 and cols and stride < cols:
-        raise ValueError(f"{name} has rows that overlap")
-    return stride
+    if step < cols:
+        if rows > 1:
+            raise ValueError(f"{name} has rows that overlap")
+        step = cols
+    return rows, cols, step, _dtype_code(name, t.dtype)
 
 
-def _id_tensor(ids, device):
-    import torch
-
-    if ids.dtype not in (torch.int32, torch.int64):
+def _id_tensor(ids, dev: int):
+    bits = _ID_BITS.get(ids.dtype)
+    if bits is None:
         raise ValueError(f"ids must be int32 or int64, not {ids.dtype}")
-    if ids.device != device:
-        raise ValueError(f"ids are on {ids.device}, not on {device}")
-    return ids.contiguous(), 32 if ids.dtype == torch.int32 else 64
+    if ids.get_device() != dev:
+        raise ValueError(f"ids are on {ids.device}, not on cuda:{dev}")
+    return (ids if ids.is_contiguous() else ids.contiguous()), bits
 
 
-def _workspace(torch, nbytes: int, device):
+def _workspace(nbytes: int, device):
     """Scratch of one call, from torch's allocator: it belongs to the current stream."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    return _torch.empty(nbytes, dtype=_torch.uint8, device=device) if nbytes else None
 
 
 def async_status(ctx: Context | None = None, device: int = 0) -> None:
     """Waits for the current stream and raises what the calls of this section left (tessa_async_status)."""
-    import torch
-
+    _lazy_torch()
     ctx = ctx or context(device)
-    C.check(C.load().tessa_async_status(ctx.handle, _stream_ptr(torch, ctx.device)))
+    C.check(C.load().tessa_async_status(ctx.handle, _stream(ctx.device)))
 
 
 def embedding_lookup(table, ids, scale: float = 1.0, out=None, out_dtype=None, ctx: Context | None = None):
@@ -853,27 +877,24 @@ def embedding_lookup(table, ids, scale: float = 1.0, out=None, out_dtype=None, c
     any shape, -1 = padding (a row of zeros).  Returns ids.shape + (dim,) in
     out_dtype (default the table's), or fills out [ids.numel(), dim].
     """
-    import torch
-
-    stride = _matrix("table", table)
-    dev = table.device
+    torch = _lazy_torch()
+    rows, dim, stride, code = _matrix("table", table)
+    dev = table.get_device()
     flat, id_bits = _id_tensor(ids, dev)
-    n, dim = flat.numel(), table.shape[1]
+    n = flat.numel()
     if out is None:
-        res = torch.empty(ids.shape + (dim,), dtype=out_dtype or table.dtype, device=dev)
-        out, out_stride = res, dim
+        res = torch.empty((*ids.shape, dim), dtype=out_dtype or table.dtype, device=table.device)
+        out_stride, out_code = dim, code if out_dtype is None else _dtype_code("out", out_dtype)
     else:
         if tuple(out.shape) != (n, dim):
             raise ValueError(f"out has shape {tuple(out.shape)}, not {(n, dim)}")
         if out_dtype is not None and out.dtype != out_dtype:
             raise ValueError(f"out is {out.dtype}, not {out_dtype}")
-        out_stride = _matrix("out", out, dev)
+        _, _, out_stride, out_code = _matrix("out", out, dev)
         res = out
-    ctx = ctx or context(dev.index)
-    a = C.LookupArgs(table.data_ptr(), table.shape[0], stride, dim, _dtype_code("table", table.dtype),
-                     flat.data_ptr(), id_bits, _dtype_code("out", out.dtype), n, float(scale), out.data_ptr(),
-                     out_stride)
-    C.check(C.load().tessa_embedding_lookup(ctx.handle, ctypes.byref(a), _stream_ptr(torch, dev.index)))
+    a = C.LookupArgs(table.data_ptr(), rows, stride, dim, code, flat.data_ptr(), id_bits, out_code, n, scale,
+                     res.data_ptr(), out_stride)
+    C.check(C.load().tessa_embedding_lookup((ctx or context(dev)).handle, a, _stream(dev)))
     return res
 
 
@@ -888,35 +909,32 @@ def embedding_grad(dout, ids, table_rows: int, scale: float = 1.0, out_dtype=Non
     out, fills it; with accumulate, adds to it and leaves the rows that no id
     names as they are.
     """
-    import torch
-
-    dev = dout.device
-    dim = dout.shape[-1]
+    torch = _lazy_torch()
+    d2 = dout if dout.dim() == 2 else dout.reshape(-1, dout.shape[-1])
+    d_rows, dim, stride, code = _matrix("dout", d2)
+    dev = d2.get_device()
     flat, id_bits = _id_tensor(ids, dev)
     n = flat.numel()
-    d2 = dout if dout.dim() == 2 else dout.reshape(-1, dim)
-    if d2.shape[0] != n:
-        raise ValueError(f"dout has {d2.shape[0]} rows for {n} ids")
-    stride = _matrix("dout", d2)
+    if d_rows != n:
+        raise ValueError(f"dout has {d_rows} rows for {n} ids")
+    table_rows = int(table_rows)
     if accumulate and out is None:
         raise ValueError("accumulate needs out")
     if out is None:
-        out = torch.empty((int(table_rows), dim), dtype=out_dtype or dout.dtype, device=dev)
-    elif tuple(out.shape) != (int(table_rows), dim):
-        raise ValueError(f"out has shape {tuple(out.shape)}, not {(int(table_rows), dim)}")
+        out = torch.empty((table_rows, dim), dtype=out_dtype or dout.dtype, device=dout.device)
+    elif tuple(out.shape) != (table_rows, dim):
+        raise ValueError(f"out has shape {tuple(out.shape)}, not {(table_rows, dim)}")
     elif out_dtype is not None and out.dtype != out_dtype:
         raise ValueError(f"out is {out.dtype}, not {out_dtype}")
-    out_stride = _matrix("out", out, dev)
+    _, _, out_stride, out_code = _matrix("out", out, dev)
     lib = C.load()
     need = ctypes.c_uint64()
-    C.check(lib.tessa_embedding_grad_workspace(n, out.shape[0], dim, ctypes.byref(need)))
-    ws = _workspace(torch, need.value, dev)
-    ctx = ctx or context(dev.index)
-    a = C.LookupGradArgs(d2.data_ptr(), stride, dim, _dtype_code("dout", d2.dtype), flat.data_ptr(), id_bits,
-                         _dtype_code("out", out.dtype), n, float(scale), int(bool(accumulate)), out.data_ptr(),
-                         out_stride, out.shape[0])
-    C.check(lib.tessa_embedding_grad(ctx.handle, ctypes.byref(a), _ptr(ws), need.value,
-                                     _stream_ptr(torch, dev.index)))
+    C.check(lib.tessa_embedding_grad_workspace(n, table_rows, dim, need))
+    ws = _workspace(need.value, dout.device)
+    a = C.LookupGradArgs(d2.data_ptr(), stride, dim, code, flat.data_ptr(), id_bits, out_code, n, scale,
+                         1 if accumulate else 0, out.data_ptr(), out_stride, table_rows)
+    C.check(lib.tessa_embedding_grad((ctx or context(dev)).handle, a, ws.data_ptr() if ws is not None else None,
+                                     need.value, _stream(dev)))
     return out
 
 
@@ -926,22 +944,21 @@ def _fp8_shape(rows: int, cols: int):
 
 
 def _quantize_fp8(x, along_rows: bool, along_cols: bool, ctx):
-    import torch
-
-    stride = _matrix("x", x)
-    dev = x.device
-    rows, cols = x.shape
-    res = []
-    for wanted, shape in ((along_rows, (rows, cols)), (along_cols, (cols, rows))):
-        if wanted:
-            c, s = _fp8_shape(*shape)
-            res += [torch.empty(c, dtype=torch.float8_e4m3fn, device=dev), torch.empty(s, dtype=torch.uint8, device=dev)]
-        else:
-            res += [None, None]
-    ctx = ctx or context(dev.index)
-    a = C.Fp8QuantizeArgs(x.data_ptr(), rows, cols, stride, _dtype_code("x", x.dtype), 0, *(_ptr(t).value for t in res))
-    C.check(C.load().tessa_quantize_fp8(ctx.handle, ctypes.byref(a), _stream_ptr(torch, dev.index)))
-    return res
+    torch = _lazy_torch()
+    rows, cols, stride, code = _matrix("x", x)
+    dev = x.get_device()
+    device, f8, u8 = x.device, torch.float8_e4m3fn, torch.uint8
+    c = s = ct = st = None
+    if along_rows:
+        cs, ss = _fp8_shape(rows, cols)
+        c, s = torch.empty(cs, dtype=f8, device=device), torch.empty(ss, dtype=u8, device=device)
+    if along_cols:
+        cs, ss = _fp8_shape(cols, rows)
+        ct, st = torch.empty(cs, dtype=f8, device=device), torch.empty(ss, dtype=u8, device=device)
+    a = C.Fp8QuantizeArgs(x.data_ptr(), rows, cols, stride, code, 0, *((c.data_ptr(), s.data_ptr()) if along_rows else (None, None)),
+                          *((ct.data_ptr(), st.data_ptr()) if along_cols else (None, None)))
+    C.check(C.load().tessa_quantize_fp8((ctx or context(dev)).handle, a, _stream(dev)))
+    return c, s, ct, st
 
 
 def quantize_fp8(x, transpose: bool = False, ctx: Context | None = None):
@@ -954,25 +971,25 @@ def quantize_fp8(x, transpose: bool = False, ctx: Context | None = None):
     blocks down the columns.
     """
     res = _quantize_fp8(x, not transpose, transpose, ctx)
-    return tuple(res[2:] if transpose else res[:2])
+    return res[2:] if transpose else res[:2]
 
 
 def quantize_fp8_both(x, ctx: Context | None = None):
     """(codes, scales, codes_t, scales_t): both forms of :func:`quantize_fp8`
     from one read of x, as a product and its gradients need them."""
-    return tuple(_quantize_fp8(x, True, True, ctx))
+    return _quantize_fp8(x, True, True, ctx)
 
 
 def _fp8_operand(name: str, codes, scales):
-    import torch
-
-    if codes.dtype not in (torch.float8_e4m3fn, torch.uint8) or scales.dtype != torch.uint8:
+    """Checks one operand; returns (rows, width)."""
+    if codes.dtype not in (_torch.float8_e4m3fn, _torch.uint8) or scales.dtype != _torch.uint8:
         raise ValueError(f"{name}: codes must be float8_e4m3fn (or its bytes) and scales uint8")
     if codes.dim() != 2 or not codes.is_cuda or not codes.is_contiguous() or not scales.is_contiguous():
         raise ValueError(f"{name}: codes and scales must be contiguous 2-D CUDA tensors")
-    want = _fp8_shape(codes.shape[0], codes.shape[1])
-    if tuple(codes.shape) != want[0] or tuple(scales.shape) != want[1] or scales.device != codes.device:
+    rows, width = codes.shape
+    if width % 16 or tuple(scales.shape) != (rows, (width + 511) // 512 * 4) or scales.get_device() != codes.get_device():
         raise ValueError(f"{name}: scales {tuple(scales.shape)} do not fit codes {tuple(codes.shape)}")
+    return rows, width
 
 
 def matmul_fp8(a_codes, a_scales, b_codes, b_scales, out_dtype=None, out=None, ctx: Context | None = None):
@@ -982,61 +999,58 @@ def matmul_fp8(a_codes, a_scales, b_codes, b_scales, out_dtype=None, out=None, c
     Operands as :func:`quantize_fp8` returns them, of the same width.  Returns
     [m, n] in out_dtype (default float32), or fills out (any row stride).
     """
-    import torch
-
-    _fp8_operand("a", a_codes, a_scales)
-    _fp8_operand("b", b_codes, b_scales)
-    dev = a_codes.device
-    m, k = a_codes.shape
-    n = b_codes.shape[0]
-    if b_codes.shape[1] != k or b_codes.device != dev:
-        raise ValueError(f"operands of {tuple(a_codes.shape)} on {dev} and {tuple(b_codes.shape)} on {b_codes.device}")
+    torch = _lazy_torch()
+    m, k = _fp8_operand("a", a_codes, a_scales)
+    n, kb = _fp8_operand("b", b_codes, b_scales)
+    dev = a_codes.get_device()
+    if kb != k or b_codes.get_device() != dev:
+        raise ValueError(f"operands of {tuple(a_codes.shape)} on {a_codes.device} and {tuple(b_codes.shape)} on "
+                         f"{b_codes.device}")
     if out is None:
-        out = torch.empty((m, n), dtype=out_dtype or torch.float32, device=dev)
+        out = torch.empty((m, n), dtype=out_dtype or torch.float32, device=a_codes.device)
     elif tuple(out.shape) != (m, n) or (out_dtype is not None and out.dtype != out_dtype):
         raise ValueError(f"out must be {(m, n)}" + (f" of {out_dtype}" if out_dtype is not None else ""))
-    out_stride = _matrix("out", out, dev)
+    _, _, out_stride, out_code = _matrix("out", out, dev)
     lib = C.load()
-    ctx = ctx or context(dev.index)
+    handle = (ctx or context(dev)).handle
     need = ctypes.c_uint64()
-    C.check(lib.tessa_matmul_fp8_workspace(ctx.handle, m, n, k, ctypes.byref(need)))
-    ws = _workspace(torch, need.value, dev)
+    C.check(lib.tessa_matmul_fp8_workspace(handle, m, n, k, need))
+    ws = _workspace(need.value, a_codes.device)
     a = C.Fp8MatmulArgs(a_codes.data_ptr(), a_scales.data_ptr(), b_codes.data_ptr(), b_scales.data_ptr(), m, n, k,
-                        out.data_ptr(), out_stride, _dtype_code("out", out.dtype), 0)
-    C.check(lib.tessa_matmul_fp8(ctx.handle, ctypes.byref(a), _ptr(ws), need.value, _stream_ptr(torch, dev.index)))
+                        out.data_ptr(), out_stride, out_code, 0)
+    C.check(lib.tessa_matmul_fp8(handle, a, ws.data_ptr() if ws is not None else None, need.value, _stream(dev)))
     return out
 
 
-def _distill(logits, teacher_ids, teacher_logits, temperature, row_weights, want_stats, want_grad, out, ctx):
-    import torch
-
-    stride = _matrix("logits", logits)
-    dev = logits.device
-    rows, vocab = logits.shape
+def _distill(logits, teacher_ids, teacher_logits, temperature, row_weights, want_grad, out, ctx):
+    torch = _lazy_torch()
+    rows, vocab, stride, code = _matrix("logits", logits)
+    dev, device = logits.get_device(), logits.device
     if teacher_ids.dim() != 2 or teacher_ids.shape[0] != rows or teacher_logits.shape != teacher_ids.shape:
         raise ValueError(f"teacher_ids {tuple(teacher_ids.shape)} and teacher_logits {tuple(teacher_logits.shape)} "
                          f"must both be [{rows}, k]")
     ids, id_bits = _id_tensor(teacher_ids, dev)
-    if not teacher_logits.is_floating_point() or teacher_logits.device != dev:
+    if not teacher_logits.is_floating_point() or teacher_logits.get_device() != dev:
         raise ValueError("teacher_logits must be floating point and on the logits' device")
     tl = teacher_logits.to(torch.float32).contiguous()
     if row_weights is not None:
-        if tuple(row_weights.shape) != (rows,) or row_weights.device != dev:
+        if tuple(row_weights.shape) != (rows,) or row_weights.get_device() != dev:
             raise ValueError(f"row_weights must be [{rows}] on the logits' device")
         row_weights = row_weights.to(torch.float32).contiguous()
-    loss = torch.empty(rows, dtype=torch.float32, device=dev) if want_stats else None
-    lse = torch.empty(rows, dtype=torch.float32, device=dev) if want_stats else None
-    grad, grad_stride = None, 0
+    stats = torch.empty((2, rows), dtype=torch.float32, device=device)
+    loss, lse = stats.unbind(0)
+    grad, grad_ptr, grad_stride = None, None, 0
     if want_grad:
-        grad = torch.empty((rows, vocab), dtype=logits.dtype, device=dev) if out is None else out
+        grad = torch.empty((rows, vocab), dtype=logits.dtype, device=device) if out is None else out
         if tuple(grad.shape) != (rows, vocab) or grad.dtype != logits.dtype:
             raise ValueError(f"out must be {(rows, vocab)} of {logits.dtype}")
-        grad_stride = _matrix("out", grad, dev)
-    ctx = ctx or context(dev.index)
-    a = C.DistillArgs(logits.data_ptr(), rows, vocab, stride, _dtype_code("logits", logits.dtype), ids.shape[1],
-                      ids.data_ptr(), tl.data_ptr(), id_bits, float(temperature), _ptr(row_weights).value,
-                      _ptr(loss).value, _ptr(lse).value, _ptr(grad).value, grad_stride)
-    C.check(C.load().tessa_distill_topk(ctx.handle, ctypes.byref(a), _stream_ptr(torch, dev.index)))
+        grad_stride = _matrix("out", grad, dev)[2]
+        grad_ptr = grad.data_ptr()
+    base = stats.data_ptr()
+    a = C.DistillArgs(logits.data_ptr(), rows, vocab, stride, code, ids.shape[1], ids.data_ptr(), tl.data_ptr(), id_bits,
+                      temperature, None if row_weights is None else row_weights.data_ptr(), base, base + 4 * rows,
+                      grad_ptr, grad_stride)
+    C.check(C.load().tessa_distill_topk((ctx or context(dev)).handle, a, _stream(dev)))
     return loss, lse, grad
 
 
@@ -1049,7 +1063,7 @@ def distill_topk(logits, teacher_ids, teacher_logits, temperature: float = 1.0, 
     temperature) over the whole row, returns (loss f32 [rows], temperature^2 *
     KL(p || q), and lse f32 [rows], log-sum-exp of logits / temperature).
     """
-    loss, lse, _ = _distill(logits, teacher_ids, teacher_logits, temperature, None, True, False, None, ctx)
+    loss, lse, _ = _distill(logits, teacher_ids, teacher_logits, temperature, None, False, None, ctx)
     return loss, lse
 
 
@@ -1061,4 +1075,4 @@ def distill_topk_grad(logits, teacher_ids, teacher_logits, temperature: float = 
     Returns (loss, lse, grad [rows, vocab] in the logits' type).  out receives
     the gradient; it may be the logits themselves.
     """
-    return _distill(logits, teacher_ids, teacher_logits, temperature, row_weights, True, True, out, ctx)
+    return _distill(logits, teacher_ids, teacher_logits, temperature, row_weights, True, out, ctx)
