@@ -813,7 +813,10 @@ typedef struct tessa_distill_args {
   void* grad;                   /* rows x vocab, or NULL */
   uint64_t grad_stride;
 } tessa_distill_args;
-TESSA_API int tessa_distill_topk(tessa_ctx* ctx, const tessa_distill_args* args, void* stream);
+/* Scratch of a call with these arguments (pointers are looked at for NULL only); may be 0. */
+TESSA_API int tessa_distill_topk_workspace(const tessa_distill_args* args, uint64_t* bytes);
+TESSA_API int tessa_distill_topk(tessa_ctx* ctx, const tessa_distill_args* args, void* workspace,
+                                 uint64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -261,7 +261,9 @@ SIGNATURES = [
     ("tessa_embedding_grad_workspace", ctypes.c_int,
      [ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint32, ctypes.POINTER(ctypes.c_uint64)]),
     ("tessa_embedding_grad", ctypes.c_int, [c_vp, ctypes.POINTER(LookupGradArgs), c_vp, ctypes.c_uint64, c_vp]),
-    ("tessa_distill_topk", ctypes.c_int, [c_vp, ctypes.POINTER(DistillArgs), c_vp]),
+    ("tessa_distill_topk_workspace", ctypes.c_int,
+     [ctypes.POINTER(DistillArgs), ctypes.POINTER(ctypes.c_uint64)]),
+    ("tessa_distill_topk", ctypes.c_int, [c_vp, ctypes.POINTER(DistillArgs), c_vp, ctypes.c_uint64, c_vp]),
     ("tessa_quantize_fp8", ctypes.c_int, [c_vp, ctypes.POINTER(Fp8QuantizeArgs), c_vp]),
     ("tessa_matmul_fp8_workspace", ctypes.c_int,
      [c_vp, ctypes.c_uint64, ctypes.c_uint64, ctypes.c_uint64, ctypes.POINTER(ctypes.c_uint64)]),

@@ -164,7 +164,15 @@ int tessa_matmul_fp8(tessa_ctx* ctx, const tessa_fp8_matmul_args* args, void* wo
   return launched("FP8 product", launch_matmul_fp8(a, workspace, c, (cudaStream_t)stream));
 }
 
-int tessa_distill_topk(tessa_ctx* ctx, const tessa_distill_args* args, void* stream) {
+int tessa_distill_topk_workspace(const tessa_distill_args* args, uint64_t* bytes) {
+  if (!args || !bytes) return bad(TESSA_ERR_INVALID_ARG, "null argument");
+  TRY(check_dtype("logits", args->dtype));
+  *bytes = distill_workspace(args->rows, args->vocab, args->dtype, args->k, args->grad != nullptr);
+  return TESSA_OK;
+}
+
+int tessa_distill_topk(tessa_ctx* ctx, const tessa_distill_args* args, void* workspace, uint64_t workspace_bytes,
+                       void* stream) {
   if (!ctx || !args) return bad(TESSA_ERR_INVALID_ARG, "null argument");
   const tessa_distill_args& a = *args;
   TRY(check_matrix("logits", a.logits, a.rows, a.vocab, a.stride, a.dtype));
@@ -178,10 +186,11 @@ int tessa_distill_topk(tessa_ctx* ctx, const tessa_distill_args* args, void* str
   if (a.rows * a.k && !a.teacher_logits) return bad(TESSA_ERR_INVALID_ARG, "teacher logits: null pointer");
   if (!(a.temperature > 0.0f) || a.temperature > 3.0e38f)
     return bad(TESSA_ERR_INVALID_ARG, "temperature %g: a positive number", (double)a.temperature);
+  TRY(check_workspace(workspace, workspace_bytes, distill_workspace(a.rows, a.vocab, a.dtype, a.k, a.grad != nullptr)));
   AsyncCtx c;
   TRY(async_begin(ctx, &c));
   if (a.rows == 0) return TESSA_OK;
-  return launched("distillation", launch_distill(a, c, (cudaStream_t)stream));
+  return launched("distillation", launch_distill(a, workspace, c, (cudaStream_t)stream));
 }
 
 }  // extern "C"

@@ -258,7 +258,8 @@ cudaError_t launch_quantize_fp8(const tessa_fp8_quantize_args& a, const AsyncCtx
 uint64_t fp8_matmul_workspace(uint64_t m, uint64_t n, uint64_t k, int sm_count);
 cudaError_t launch_matmul_fp8(const tessa_fp8_matmul_args& a, void* workspace, const AsyncCtx& c,
                               cudaStream_t stream);
-cudaError_t launch_distill(const tessa_distill_args& a, const AsyncCtx& c, cudaStream_t stream);
+uint64_t distill_workspace(uint64_t rows, uint64_t vocab, uint32_t dtype, uint32_t k, bool grad);
+cudaError_t launch_distill(const tessa_distill_args& a, void* workspace, const AsyncCtx& c, cudaStream_t stream);
 // 2-D uint8 tensor map (leaf_sq8.cu): rows x row_bytes, box of 128 bytes x
 // box_rows, 128-byte swizzle, zero fill.
 int make_code_tmap(CUtensorMap* map, const void* base, uint64_t rows, uint32_t row_bytes, uint32_t box_rows);

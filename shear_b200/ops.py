@@ -1050,7 +1050,12 @@ def _distill(logits, teacher_ids, teacher_logits, temperature, row_weights, want
     a = C.DistillArgs(logits.data_ptr(), rows, vocab, stride, code, ids.shape[1], ids.data_ptr(), tl.data_ptr(), id_bits,
                       temperature, None if row_weights is None else row_weights.data_ptr(), base, base + 4 * rows,
                       grad_ptr, grad_stride)
-    C.check(C.load().tessa_distill_topk((ctx or context(dev)).handle, a, _stream(dev)))
+    lib, ws, need = C.load(), None, ctypes.c_uint64()
+    if want_grad:
+        C.check(lib.tessa_distill_topk_workspace(a, need))
+        ws = _workspace(need.value, device)
+    C.check(lib.tessa_distill_topk((ctx or context(dev)).handle, a, ws.data_ptr() if ws is not None else None,
+                                   need.value, _stream(dev)))
     return loss, lse, grad
 
 
