@@ -47,10 +47,11 @@ constexpr uint64_t kGivenUpNs = 1000000ull;  // for what is still under way afte
 constexpr uint32_t kScaleWarp = 4, kEpiWarp = 8;
 
 struct Params {
-  const uint8_t* p_scales;  // a's
-  const uint8_t* q_scales;  // b's
+  const uint8_t* p_scales;  // of the operand in the accumulator's lanes: a, or b where swapped
+  const uint8_t* q_scales;  // of the other
   uint64_t scale_cols;
-  uint64_t m, n;
+  uint64_t rows_p, rows_q;  // m and n, or n and m where the operands are swapped
+  uint64_t m;
   uint32_t kblocks;         // blocks of 128
   uint32_t ksteps;          // steps of 32 that hold data
   uint32_t bn;
@@ -62,7 +63,6 @@ struct Params {
   uint64_t out_stride;
   float* parts;             // splits x m x parts_stride, splits > 1
   uint64_t parts_stride;    // n rounded up to 4
-  uint32_t tma_out;         // out's rows suit TMA (16-byte base and stride); parts' always do
   uint32_t* err;
   uint64_t timeout_ns;
 };
@@ -209,6 +209,25 @@ __device__ __forceinline__ void span_of(const Params& p, uint32_t u, uint32_t& k
   }
 }
 
+// Accumulator columns of the lane's place: out[i * stride], i < rows.  Four
+// pointers, so that a store does not wait for the address of the one before.
+template <class O>
+__device__ __forceinline__ void store32(O* out, uint64_t stride, const uint32_t (&v)[32], uint32_t rows) {
+  O *p0 = out, *p1 = out + stride, *p2 = p1 + stride, *p3 = p2 + stride;
+  const uint64_t step = 4u * stride;
+#pragma unroll
+  for (uint32_t i = 0; i < 32; i += 4) {
+    if (i < rows) *p0 = from_f32<O>(__uint_as_float(v[i]));
+    if (i + 1u < rows) *p1 = from_f32<O>(__uint_as_float(v[i + 1]));
+    if (i + 2u < rows) *p2 = from_f32<O>(__uint_as_float(v[i + 2]));
+    if (i + 3u < rows) *p3 = from_f32<O>(__uint_as_float(v[i + 3]));
+    p0 += step;
+    p1 += step;
+    p2 += step;
+    p3 += step;
+  }
+}
+
 // 128 bytes of a row (32 f32 or 64 16-bit columns) of the accumulator as eight
 // 16-byte pieces.
 template <class O>
@@ -232,7 +251,7 @@ __device__ __forceinline__ void load_row(uint32_t taddr, uint4 (&piece)[8]) {
   }
 }
 
-template <class O, bool PARTS>
+template <class O, bool PARTS, bool SWAP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fp8_matmul_kernel(const __grid_constant__ CUtensorMap pmap, const __grid_constant__ CUtensorMap qmap,
                       const __grid_constant__ CUtensorMap omap, const Params p) {
@@ -420,9 +439,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const uint64_t pr = (uint64_t)(t.p * 2u + rank) * kBP + i, qr = (uint64_t)t.q * p.bn + i;
       kb = t.kb0;
       kb1 = t.kb1;
-      has_p = pr < p.m;
-      has_q = i < p.bn && qr < p.n;
-      has_r = i + 128u < p.bn && qr + 128u < p.n;
+      has_p = pr < p.rows_p;
+      has_q = i < p.bn && qr < p.rows_q;
+      has_r = i + 128u < p.bn && qr + 128u < p.rows_q;
       src_p = p.p_scales + (has_p ? pr : 0u) * p.scale_cols;
       src_q = p.q_scales + (has_q ? qr : 0u) * p.scale_cols;
       src_r = p.q_scales + (has_r ? qr + 128u : 0u) * p.scale_cols;
@@ -484,7 +503,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp >= kEpiWarp) {
     // Two warps a lane quadrant take turns at 128 bytes of its rows.
     const uint32_t quad = warp % 4u, turn = (warp - kEpiWarp) / 4u;
-    uint8_t* boxes = smem + p.stages * stage_bytes + (warp - kEpiWarp) * kBoxes * kBoxBytes;
+    [[maybe_unused]] uint8_t* boxes = smem + p.stages * stage_bytes + (warp - kEpiWarp) * kBoxes * kBoxBytes;
     uint32_t acc = 0;
     for (uint32_t u = unit0; u < units; u += ustep, ++acc) {
       const Unit t = unit_of(p, u);
@@ -492,61 +511,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const bool full_ok = lane != 0 || wait(&acc_full[buf], (acc >> 1) & 1u);
       if (!__shfl_sync(0xffffffffu, full_ok ? 1u : 0u, 0)) break;
       tc_fence_after();
-      constexpr uint32_t kCols = 64u / sizeof(O);  // of a box, two boxes a turn; BN is a multiple of 32
-      const uint64_t m0 = (uint64_t)(t.p * 2u + rank) * kBP + quad * 32u, n0 = (uint64_t)t.q * p.bn;
-      const uint32_t cols = m0 < p.m ? (uint32_t)min((uint64_t)p.bn, p.n - n0) : 0u;
-      const uint32_t rows = m0 < p.m ? (uint32_t)min((uint64_t)32u, p.m - m0) : 0u;
+      const uint64_t p0 = (uint64_t)(t.p * 2u + rank) * kBP + quad * 32u, q0 = (uint64_t)t.q * p.bn;
+      const uint32_t rows = p0 < p.rows_p ? (uint32_t)min((uint64_t)32u, p.rows_p - p0) : 0u;
+      const uint32_t cols = rows ? (uint32_t)min((uint64_t)p.bn, p.rows_q - q0) : 0u;
       const uint32_t ta = tmem + buf * kMaxBN + (quad << 21);  // lane quad * 32
-      O* out;
-      uint64_t stride;
-      if constexpr (PARTS) {
-        out = reinterpret_cast<O*>(p.parts) + ((uint64_t)t.split * p.m + m0) * p.parts_stride + n0;
-        stride = p.parts_stride;
-      } else {
-        out = static_cast<O*>(p.out) + m0 * p.out_stride + n0;
-        stride = p.out_stride;
-      }
-      for (uint32_t c = turn * 2u * kCols; c < cols; c += 4u * kCols) {
-        uint4 piece[8];
-        load_row<O>(ta + c, piece);  // may read past BN into other columns of the allocation
-        const uint32_t width = min(2u * kCols, cols - c);
-        if ((PARTS || p.tma_out) && rows <= 4u && width == 2u * kCols) {
-          // few rows: sixteen bytes at a time, sooner done than a store by TMA
-          if (lane < rows) {
-            uint4* dst = reinterpret_cast<uint4*>(out + lane * stride + c);
-#pragma unroll
-            for (uint32_t j = 0; j < 8; ++j) dst[j] = piece[j];
-          }
+      O* out = PARTS ? reinterpret_cast<O*>(p.parts) + (uint64_t)t.split * p.m * p.parts_stride : static_cast<O*>(p.out);
+      const uint64_t stride = PARTS ? p.parts_stride : p.out_stride;
+      if constexpr (SWAP) {
+        // A column of the accumulator is 32 neighbours of one row of out.
+        out += q0 * stride + p0 + lane;
+        for (uint32_t c = turn * 32u; c < cols; c += 64u) {
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(ta + c, v);  // BN is a multiple of 32
+          tmem_ld_wait();
+          if (lane < rows) store32(out + c * stride, stride, v, cols - c);
           __syncwarp();  // the next load is the whole warp's
-          continue;
         }
-        // the last stores out of the boxes have read them
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        __syncwarp();
+      } else {
+        constexpr uint32_t kCols = 64u / sizeof(O);  // of a box, two boxes a turn
+        for (uint32_t c = turn * 2u * kCols; c < cols; c += 4u * kCols) {
+          uint4 piece[8];
+          load_row<O>(ta + c, piece);  // may read past BN into other columns of the allocation
+          // the last stores out of the boxes have read them
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          __syncwarp();
 #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j)
-          *reinterpret_cast<uint4*>(boxes + j / 4u * kBoxBytes + lane * 64u + ((j ^ (lane >> 1)) & 3u) * 16u) = piece[j];
-        if (PARTS || p.tma_out) {  // out's right and lower edges TMA cuts
+          for (uint32_t j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(boxes + j / 4u * kBoxBytes + lane * 64u + ((j ^ (lane >> 1)) & 3u) * 16u) =
+                piece[j];
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) {
-            store_box(&omap, smem_u32(boxes), (int32_t)(n0 + c), (int32_t)m0, (int32_t)t.split);
-            if (width > kCols)
-              store_box(&omap, smem_u32(boxes) + kBoxBytes, (int32_t)(n0 + c + kCols), (int32_t)m0, (int32_t)t.split);
+          if (lane == 0) {  // out's right and lower edges TMA cuts
+            store_box(&omap, smem_u32(boxes), (int32_t)(q0 + c), (int32_t)p0, (int32_t)t.split);
+            if (cols - c > kCols)
+              store_box(&omap, smem_u32(boxes) + kBoxBytes, (int32_t)(q0 + c + kCols), (int32_t)p0, (int32_t)t.split);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
-        } else {
-          __syncwarp();
-          constexpr uint32_t kPiece = 16u / sizeof(O);  // columns of a piece
-          for (uint32_t k = lane; k < width; k += 32u) {
-            const uint8_t* box = boxes + k / kCols * kBoxBytes;
-            const uint32_t j = k % kCols / kPiece;
-            O* dst = out + c + k;
-#pragma unroll 8
-            for (uint32_t r = 0; r < rows; ++r, dst += stride)
-              *dst = reinterpret_cast<const O*>(box + r * 64u + ((j ^ (r >> 1)) & 3u) * 16u)[k % kPiece];
-          }
-          __syncwarp();
         }
       }
       tc_fence_before();
@@ -606,29 +606,33 @@ struct Plan {
 // pair: a block of K takes 2 BN cycles of the tensor cores (156 at least: the
 // four MMAs' issue), a tile about 1500 beside its MMAs, a split its parts'
 // traffic and a second launch.
-inline Plan plan(uint64_t m, uint64_t n, uint64_t k, int sm_count) {
+inline Plan plan(uint64_t rows_p, uint64_t rows_q, uint64_t k, int sm_count) {
   Plan best = {};
   double best_cost = 0.0;
   const uint32_t pairs = (uint32_t)sm_count / 2u;
-  const uint32_t groups = (uint32_t)div_up(k, 512), tp = (uint32_t)div_up(m, 2 * kBP);
-  const uint64_t least = div_up(n, kMaxBN);
+  const uint32_t groups = (uint32_t)div_up(k, 512), tp = (uint32_t)div_up(rows_p, 2 * kBP);
+  const uint64_t least = div_up(rows_q, kMaxBN);
+  // The tensor core cuts each sum's low bits, always towards zero: 4096 terms
+  // of one sign end up 1.4e-6 off, and it grows with their number.  Parts of at
+  // most 8192 terms are added with full rounding.
+  const uint32_t fewest = (uint32_t)div_up(groups, 16);
   // tile counts that fill whole rounds of the SM pairs, and the fewest
   const uint64_t wave = pairs / tp ? pairs / tp : 1;
   for (uint64_t i = 0; i < 12; ++i) {
     const uint64_t tq = i < 8 ? least + i : div_up(least, wave) * wave + (i - 8) * wave;
-    if (tq > div_up(n, 32)) continue;
-    const uint32_t bn = (uint32_t)(div_up(div_up(n, tq), 32) * 32);
-    if (div_up(n, bn) != tq) continue;
+    if (tq > div_up(rows_q, 32)) continue;
+    const uint32_t bn = (uint32_t)(div_up(div_up(rows_q, tq), 32) * 32);
+    if (div_up(rows_q, bn) != tq) continue;
     // splitting pays only while whole tiles leave SMs without work
     const uint32_t most = (uint64_t)tp * tq >= (uint64_t)pairs ? 1u : 32u;
-    for (uint32_t want = 1; want <= groups && want <= most; ++want) {
+    for (uint32_t want = fewest; want <= groups && (want <= most || want == fewest); ++want) {
       const uint32_t sg = (uint32_t)div_up(groups, want), splits = (uint32_t)div_up(groups, sg);
       if (splits != want) continue;
       const uint64_t units = (uint64_t)tp * tq * splits;
-      if (splits > 1 && units > 2 * pairs) break;
+      if (want > fewest && units > 2 * pairs) break;
       const double blocks = sg * 4.0 < (double)div_up(k, 128) ? sg * 4.0 : (double)div_up(k, 128);
       double cost = (double)div_up(units, pairs) * (blocks * (2.0 * bn > 156.0 ? 2.0 * bn : 156.0) + 1500.0);
-      if (splits > 1) cost += 5000.0 + 8.0 * splits * (double)m * (double)n / 3500.0;
+      if (splits > 1) cost += 5000.0 + 8.0 * splits * (double)rows_p * (double)rows_q / 3500.0;
       if (best.bn == 0 || cost < best_cost) {
         best = {bn, tp, (uint32_t)tq, splits, sg};
         best_cost = cost;
@@ -640,31 +644,31 @@ inline Plan plan(uint64_t m, uint64_t n, uint64_t k, int sm_count) {
 
 // The plan of the calling thread's last few shapes (the search takes longer
 // than a launch).
-inline Plan plan_of(uint64_t m, uint64_t n, uint64_t k, int sm_count) {
+inline Plan plan_of(uint64_t rows_p, uint64_t rows_q, uint64_t k, int sm_count) {
   struct Entry {
-    uint64_t m = 0, n = 0, k = 0;
+    uint64_t p = 0, q = 0, k = 0;
     int sms = 0;
     Plan plan;
   };
   thread_local Entry kept[16];
-  Entry& e = kept[(m * 31 + n * 7 + k / 16) % 16];
-  if (e.m != m || e.n != n || e.k != k || e.sms != sm_count) {
-    e.plan = plan(m, n, k, sm_count);
-    e.m = m;
-    e.n = n;
+  Entry& e = kept[(rows_p * 31 + rows_q * 7 + k / 16) % 16];
+  if (e.p != rows_p || e.q != rows_q || e.k != k || e.sms != sm_count) {
+    e.plan = plan(rows_p, rows_q, k, sm_count);
+    e.p = rows_p;
+    e.q = rows_q;
     e.k = k;
     e.sms = sm_count;
   }
   return e.plan;
 }
 
-template <class O, bool PARTS>
+template <class O, bool PARTS, bool SWAP>
 cudaError_t launch(const CUtensorMap& pm, const CUtensorMap& qm, const CUtensorMap& om, const Params& p, int device, uint32_t smem,
                    uint32_t grid, cudaStream_t stream) {
   static SmemRaised raised;
-  cudaError_t e = raise_smem(fp8_matmul_kernel<O, PARTS>, device, (int)(kSmemLimit - kStatic), raised);
+  cudaError_t e = raise_smem(fp8_matmul_kernel<O, PARTS, SWAP>, device, (int)(kSmemLimit - kStatic), raised);
   if (e != cudaSuccess) return e;
-  fp8_matmul_kernel<O, PARTS><<<grid, kThreads, smem, stream>>>(pm, qm, om, p);
+  fp8_matmul_kernel<O, PARTS, SWAP><<<grid, kThreads, smem, stream>>>(pm, qm, om, p);
   return cudaGetLastError();
 }
 
@@ -672,28 +676,48 @@ cudaError_t launch(const CUtensorMap& pm, const CUtensorMap& qm, const CUtensorM
 }  // namespace train
 
 uint64_t fp8_matmul_workspace(uint64_t m, uint64_t n, uint64_t k, int sm_count) {
+  using namespace train;
   if (m == 0 || n == 0 || k == 0) return 0;
-  const train::mm::Plan pl = train::mm::plan_of(m, n, k, sm_count);
-  return pl.splits > 1 ? (uint64_t)pl.splits * m * train::div_up(n, 4) * 16 : 0;
+  const uint32_t one = mm::plan_of(m, n, k, sm_count).splits, other = mm::plan_of(n, m, k, sm_count).splits;
+  const uint32_t splits = one > other ? one : other;  // which of the two depends on out's alignment
+  return splits > 1 ? (uint64_t)splits * m * div_up(n, 4) * 16 : 0;
 }
 
 cudaError_t launch_matmul_fp8(const tessa_fp8_matmul_args& a, void* workspace, const AsyncCtx& c,
                               cudaStream_t stream) {
   using namespace train;
+  const uint32_t ob = type_bytes(a.out_dtype);
   if (a.k == 0)
-    return cudaMemset2DAsync(a.out, (a.m > 1 ? a.out_stride : a.n) * type_bytes(a.out_dtype), 0,
-                             a.n * type_bytes(a.out_dtype), a.m, stream);
-  const mm::Plan pl = mm::plan_of(a.m, a.n, a.k, c.sm_count);
+    return cudaMemset2DAsync(a.out, (a.m > 1 ? a.out_stride : a.n) * ob, 0, a.n * ob, a.m, stream);
+  // b's rows take the accumulator's lanes (then out is stored straight, 32
+  // neighbours at a time) where a has few rows, which would leave the lanes
+  // empty (against 200000 x 768, f32 scores: m = 16 takes 39 us so and 47
+  // otherwise, m = 128 54 and 55, m = 192 65 and 59), and where out's rows do
+  // not suit TMA.
   CUtensorMap pm, qm, om = {};
-  if (make_code_tmap(&pm, a.a_codes, a.m, (uint32_t)a.k, mm::kBP) != 0 ||
-      make_code_tmap(&qm, a.b_codes, a.n, (uint32_t)a.k, pl.bn / 2) != 0)
-    return cudaErrorInvalidValue;
+  bool swap = a.m <= mm::kBP;
+  mm::Plan pl = mm::plan_of(a.m, a.n, a.k, c.sm_count);
+  if (!swap && pl.splits == 1) {
+    const uint64_t stride = a.m > 1 ? a.out_stride : div_up(a.n, 8) * 8;
+    swap = reinterpret_cast<uintptr_t>(a.out) % 16 != 0 || stride * ob % 16 != 0 ||
+           make_store_tmap(&om, a.out, a.out_dtype, a.m, a.n, stride, 1) != 0;
+  }
+  if (swap) pl = mm::plan_of(a.n, a.m, a.k, c.sm_count);
   mm::Params p = {};
-  p.p_scales = a.a_scales;
-  p.q_scales = a.b_scales;
+  p.parts = static_cast<float*>(workspace);
+  p.parts_stride = div_up(a.n, 4) * 4;
+  if (!swap && pl.splits > 1 &&
+      make_store_tmap(&om, p.parts, TESSA_F32, a.m, a.n, p.parts_stride, pl.splits) != 0)
+    return cudaErrorInvalidValue;
+  p.rows_p = swap ? a.n : a.m;
+  p.rows_q = swap ? a.m : a.n;
+  if (make_code_tmap(&pm, swap ? a.b_codes : a.a_codes, p.rows_p, (uint32_t)a.k, mm::kBP) != 0 ||
+      make_code_tmap(&qm, swap ? a.a_codes : a.b_codes, p.rows_q, (uint32_t)a.k, pl.bn / 2) != 0)
+    return cudaErrorInvalidValue;
+  p.p_scales = swap ? a.b_scales : a.a_scales;
+  p.q_scales = swap ? a.a_scales : a.b_scales;
   p.scale_cols = div_up(a.k, 512) * 4;
   p.m = a.m;
-  p.n = a.n;
   p.kblocks = (uint32_t)div_up(a.k, 128);
   p.ksteps = (uint32_t)div_up(a.k, 32);
   p.bn = pl.bn;
@@ -701,45 +725,36 @@ cudaError_t launch_matmul_fp8(const tessa_fp8_matmul_args& a, void* workspace, c
   p.tiles_q = pl.tiles_q;
   p.splits = pl.splits;
   p.split_groups = pl.split_groups;
-  // one tile an SM pair, as far as 32 MB of b go
+  // one tile an SM pair, as far as 32 MB of the columns' operand go
   const uint64_t fit = (32ull << 20) / (a.k * pl.bn), pairs = (uint64_t)c.sm_count / 2;
   p.raster = (uint32_t)(fit > pairs ? pairs : fit < 8 ? 8 : fit);
-  const uint32_t stage = (mm::kBP + pl.bn / 2) * mm::kBK;
-  const uint32_t boxes = 8u * mm::kBoxes * mm::kBoxBytes;
+  const uint32_t stage = (mm::kBP + pl.bn / 2) * mm::kBK, boxes = swap ? 0u : 8u * mm::kBoxes * mm::kBoxBytes;
   p.stages = (mm::kSmemLimit - mm::kStatic - 1024u - boxes) / stage;
   if (p.stages > mm::kMaxStages) p.stages = mm::kMaxStages;
   p.out = a.out;
   p.out_stride = a.out_stride;
-  p.parts = static_cast<float*>(workspace);
-  p.parts_stride = div_up(a.n, 4) * 4;
-  if (pl.splits > 1) {
-    if (make_store_tmap(&om, p.parts, TESSA_F32, a.m, a.n, p.parts_stride, pl.splits) != 0)
-      return cudaErrorInvalidValue;
-  } else {
-    const uint32_t ob = type_bytes(a.out_dtype);
-    const uint64_t stride = a.m > 1 ? a.out_stride : div_up(a.n, 8) * 8;
-    p.tma_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && stride * ob % 16 == 0 &&
-                make_store_tmap(&om, a.out, a.out_dtype, a.m, a.n, stride, 1) == 0;
-  }
   p.err = c.err;
   p.timeout_ns = c.timeout_ns;
   const uint32_t smem = p.stages * stage + boxes + 1024u;
   const uint64_t units = (uint64_t)pl.tiles_p * pl.tiles_q * pl.splits;
   const uint32_t grid = 2u * (uint32_t)(units < pairs ? units : pairs);
-  if (pl.splits > 1) {
-    cudaError_t e = mm::launch<float, true>(pm, qm, om, p, c.device, smem, grid, stream);
-    if (e != cudaSuccess) return e;
-    const bool vec = vector_elems(a.out, a.m, a.n, a.out_stride, type_bytes(a.out_dtype), 4) == 4;
-    const dim3 blocks((uint32_t)div_up(a.n, 512), (uint32_t)(a.m < 32768 ? a.m : 32768));
+  if (pl.splits == 1)
     return with_type(a.out_dtype, [&](auto o) {
       using O = decltype(o);
-      mm::add_parts_kernel<O><<<blocks, 128, 0, stream>>>(p.parts, p.parts_stride, pl.splits, a.m, a.n,
-                                                          static_cast<O*>(a.out), a.out_stride, vec);
-      return cudaGetLastError();
+      return swap ? mm::launch<O, false, true>(pm, qm, om, p, c.device, smem, grid, stream)
+                  : mm::launch<O, false, false>(pm, qm, om, p, c.device, smem, grid, stream);
     });
-  }
-  return with_type(a.out_dtype,
-                   [&](auto o) { return mm::launch<decltype(o), false>(pm, qm, om, p, c.device, smem, grid, stream); });
+  cudaError_t e = swap ? mm::launch<float, true, true>(pm, qm, om, p, c.device, smem, grid, stream)
+                       : mm::launch<float, true, false>(pm, qm, om, p, c.device, smem, grid, stream);
+  if (e != cudaSuccess) return e;
+  const bool vec = vector_elems(a.out, a.m, a.n, a.out_stride, ob, 4) == 4;
+  const dim3 blocks((uint32_t)div_up(a.n, 512), (uint32_t)(a.m < 32768 ? a.m : 32768));
+  return with_type(a.out_dtype, [&](auto o) {
+    using O = decltype(o);
+    mm::add_parts_kernel<O><<<blocks, 128, 0, stream>>>(p.parts, p.parts_stride, pl.splits, a.m, a.n,
+                                                        static_cast<O*>(a.out), a.out_stride, vec);
+    return cudaGetLastError();
+  });
 }
 
 }  // namespace tessa
