@@ -10,7 +10,9 @@
 // tile's rows run by run in f32: a run inside the tile is written at once, a
 // run that crosses a tile border leaves its part in the workspace, and a last
 // kernel adds each such run's parts.  Every tile holds 32 entries however
-// popular one id is, so skew costs nothing but the parts.
+// popular one id is, so skew costs nothing but the parts.  Clearing the rows
+// that no id names on a second stream, beside the sort, gained nothing
+// (200000 x 128 f32 88 us either way, 1M x 768 bf16 428): it is in order.
 #include "train_common.cuh"
 
 namespace tessa {
@@ -47,8 +49,10 @@ __global__ void __launch_bounds__(256) lookup_kernel(const tessa_lookup_args a, 
 constexpr uint32_t kSortThreads = 512;
 constexpr uint32_t kSortWarps = kSortThreads / 32;
 constexpr uint32_t kMaxDigitBits = 10;
+constexpr uint32_t kBatch = 8;         // keys a thread has under way
 constexpr uint32_t kSmallSort = 2048;  // entries that one block sorts in shared memory
 constexpr uint32_t kTile = 32;         // sorted entries a warp sums
+constexpr uint32_t kLongRun = 64;      // tiles that a run goes on for, from which a block adds its parts
 
 struct SortPlan {
   uint32_t passes, digit_bits, chunk, blocks;
@@ -60,9 +64,10 @@ inline SortPlan sort_plan(uint64_t count, uint64_t table_rows) {
   SortPlan p;
   p.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
   p.digit_bits = (bits + p.passes - 1) / p.passes;
-  // 4096 entries a block, more where that would be over 256 blocks: every
-  // block reads all blocks' digit counts.
-  p.chunk = 4096u * (uint32_t)div_up(count, 4096ull * 256ull);
+  // At most 128 blocks, of a multiple of 2048 entries: every block reads all
+  // blocks' digit counts.  131072 entries, gradient of 128 f32 columns: 85 us
+  // with 2048 a block, 91 with 1024 or 4096; 524288: 167 with 4096, 183 with 2048.
+  p.chunk = 2048u * (uint32_t)div_up(count, 2048ull * 128ull);
   p.blocks = (uint32_t)div_up(count, p.chunk ? p.chunk : 1);
   return p;
 }
@@ -84,6 +89,7 @@ struct SortArgs {
   uint32_t* out_keys;
   uint32_t* out_pos;
   uint32_t* counts;       // blocks x bins
+  uint32_t* runs;         // two counters, cleared for the sums
   uint64_t table_rows;
   uint32_t count, chunk, shift, bins;
   uint32_t* err;
@@ -100,8 +106,16 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const SortArgs
   for (uint32_t b = threadIdx.x; b < a.bins; b += kSortThreads) bin[b] = 0;
   __syncthreads();
   const uint32_t lo = blockIdx.x * a.chunk, hi = min(a.count, lo + a.chunk);
-  for (uint32_t i = lo + threadIdx.x; i < hi; i += kSortThreads)
-    atomicAdd(&bin[(sort_key<FIRST>(a, i, a.err) >> a.shift) & (a.bins - 1u)], 1u);
+  if (FIRST && blockIdx.x == 0 && threadIdx.x < 2u) a.runs[threadIdx.x] = 0u;
+  for (uint32_t i = lo + threadIdx.x; i < hi; i += kBatch * kSortThreads) {
+    uint32_t key[kBatch];
+#pragma unroll
+    for (uint32_t r = 0; r < kBatch; ++r)
+      if (i + r * kSortThreads < hi) key[r] = sort_key<FIRST>(a, i + r * kSortThreads, a.err);
+#pragma unroll
+    for (uint32_t r = 0; r < kBatch; ++r)
+      if (i + r * kSortThreads < hi) atomicAdd(&bin[(key[r] >> a.shift) & (a.bins - 1u)], 1u);
+  }
   __syncthreads();
   for (uint32_t b = threadIdx.x; b < a.bins; b += kSortThreads) a.counts[(uint64_t)blockIdx.x * a.bins + b] = bin[b];
 }
@@ -145,12 +159,24 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortAr
   const uint32_t part = a.chunk / kSortWarps;  // a multiple of 32
   const uint32_t lo = min(a.count, blockIdx.x * a.chunk + warp * part), hi = min(a.count, lo + part);
   uint32_t* mine = warp_bin + warp * a.bins;
-  for (uint32_t i = lo; i < hi; i += 32) {
-    const bool in = i + lane < hi;
-    const uint32_t d = in ? (sort_key<FIRST>(a, i + lane, a.err) >> a.shift) & (a.bins - 1u) : a.bins;
-    const uint32_t same = __match_any_sync(0xffffffffu, d);
-    if (in && lane == (uint32_t)__ffs(same) - 1u) mine[d] += __popc(same);
-    __syncwarp();
+  uint32_t key[kBatch];
+  auto load = [&](uint32_t i) {
+#pragma unroll
+    for (uint32_t r = 0; r < kBatch; ++r) {
+      const uint32_t at = i + r * 32u + lane;
+      key[r] = at < hi ? sort_key<FIRST>(a, at, a.err) : 0u;
+    }
+  };
+  for (uint32_t i = lo; i < hi; i += kBatch * 32u) {
+    load(i);
+#pragma unroll
+    for (uint32_t r = 0; r < kBatch; ++r) {
+      const bool in = i + r * 32u + lane < hi;
+      const uint32_t d = in ? (key[r] >> a.shift) & (a.bins - 1u) : a.bins;
+      const uint32_t same = __match_any_sync(0xffffffffu, d);
+      if (in && lane == (uint32_t)__ffs(same) - 1u) mine[d] += __popc(same);
+      __syncwarp();
+    }
   }
   __syncthreads();
   if (2u * tid < a.bins) {
@@ -166,19 +192,28 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortAr
     }
   }
   __syncthreads();
-  for (uint32_t i = lo; i < hi; i += 32) {
-    const bool in = i + lane < hi;
-    const uint32_t key = in ? sort_key<FIRST>(a, i + lane, a.err) : 0u;
-    const uint32_t d = in ? (key >> a.shift) & (a.bins - 1u) : a.bins;
-    const uint32_t same = __match_any_sync(0xffffffffu, d);
-    const uint32_t rank = __popc(same & ((1u << lane) - 1u));
-    uint32_t place = in ? mine[d] + rank : 0u;
-    __syncwarp();
-    if (in && rank == 0) mine[d] += __popc(same);
-    __syncwarp();
-    if (in) {
-      a.out_keys[place] = key;
-      a.out_pos[place] = FIRST ? i + lane : a.pos[i + lane];
+  for (uint32_t i = lo; i < hi; i += kBatch * 32u) {
+    if (hi - lo > kBatch * 32u) load(i);  // else they are still there
+    uint32_t pos[kBatch];
+#pragma unroll
+    for (uint32_t r = 0; r < kBatch; ++r) {
+      const uint32_t at = i + r * 32u + lane;
+      pos[r] = FIRST || at >= hi ? at : a.pos[at];
+    }
+#pragma unroll
+    for (uint32_t r = 0; r < kBatch; ++r) {
+      const bool in = i + r * 32u + lane < hi;
+      const uint32_t d = in ? (key[r] >> a.shift) & (a.bins - 1u) : a.bins;
+      const uint32_t same = __match_any_sync(0xffffffffu, d);
+      const uint32_t rank = __popc(same & ((1u << lane) - 1u));
+      const uint32_t place = in ? mine[d] + rank : 0u;
+      __syncwarp();
+      if (in && rank == 0) mine[d] += __popc(same);
+      __syncwarp();
+      if (in) {
+        a.out_keys[place] = key[r];
+        a.out_pos[place] = pos[r];
+      }
     }
   }
 }
@@ -186,6 +221,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortAr
 // Few entries: one block, a bitonic sort of (key, position) in shared memory.
 __global__ void __launch_bounds__(1024) sort_small_kernel(const SortArgs a) {
   __shared__ uint64_t e[kSmallSort];
+  if (threadIdx.x < 2u) a.runs[threadIdx.x] = 0u;
   uint32_t n = 32;
   while (n < a.count) n <<= 1;
   for (uint32_t i = threadIdx.x; i < n; i += 1024u)
@@ -210,12 +246,128 @@ __global__ void __launch_bounds__(1024) sort_small_kernel(const SortArgs a) {
   }
 }
 
+// Up to 65536 entries: one cluster of CTAs sorts them in its shared memory,
+// every pass in the same launch.  A CTA has `chunk` places; a warp owns a
+// contiguous part of them.  Per pass: each warp counts its part's digits, the
+// CTAs read one another's totals, and every entry goes to its place, in
+// whichever CTA that is (the last pass: to global memory).  One launch instead
+// of two a pass, each nearly all latency: the gradient of 4096 entries takes 37
+// us instead of 59, of 65536 61 instead of 74; with 131072 on 16 SMs the
+// scattered stores weigh more, 94 instead of 91.
+constexpr uint32_t kClusterThreads = 1024, kClusterWarps = 32;
+constexpr uint32_t kClusterChunk = 4096;  // entries a CTA at most
+constexpr uint32_t kClusterMost = 16u * kClusterChunk;
+
+__global__ void __launch_bounds__(kClusterThreads)
+    sort_cluster_kernel(const SortArgs a, uint32_t ctas, uint32_t chunk_log2, uint32_t passes, uint32_t digit_bits) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const uint32_t chunk = 1u << chunk_log2, bins = 1u << digit_bits;
+  uint2* buf[2] = {reinterpret_cast<uint2*>(smem), reinterpret_cast<uint2*>(smem) + chunk};  // the second if passes > 2
+  uint16_t* warp_bin = reinterpret_cast<uint16_t*>(smem + (passes > 2u ? 2u : 1u) * chunk * 8u);  // warps x bins
+  __shared__ uint32_t hist[1u << kMaxDigitBits], first_place[1u << kMaxDigitBits];
+  __shared__ uint32_t warp_sum[kClusterWarps];
+  const uint32_t tid = threadIdx.x, warp = tid / 32u, lane = tid % 32u, rank = cluster_ctarank();
+  const uint32_t part = chunk / kClusterWarps, lo = warp * part;  // a multiple of 32 places
+  const uint32_t here = a.count > rank * chunk ? min(chunk, a.count - rank * chunk) : 0u;
+  uint16_t* mine = warp_bin + warp * bins;
+  if (rank == 0 && tid < 2u) a.runs[tid] = 0u;
+  cluster_sync();  // every CTA has started
+  for (uint32_t pass = 0; pass < passes; ++pass) {
+    const uint32_t shift = pass * digit_bits;
+    uint2 e[kBatch];  // (key, position)
+#pragma unroll
+    for (uint32_t r = 0; r < kBatch; ++r) {
+      const uint32_t i = lo + r * 32u + lane;
+      e[r] = make_uint2(0u, 0u);
+      if (r * 32u < part && i < here) {
+        const uint32_t at = rank * chunk + i;
+        e[r] = pass ? buf[(pass - 1u) & 1u][i] : make_uint2(id_key(a.ids, a.id_bits, at, a.table_rows, a.err), at);
+      }
+    }
+    for (uint32_t i = lane; i < bins; i += 32u) mine[i] = 0;
+    __syncwarp();
+#pragma unroll
+    for (uint32_t r = 0; r < kBatch; ++r) {
+      if (r * 32u >= part) break;
+      const bool in = lo + r * 32u + lane < here;
+      const uint32_t d = in ? (e[r].x >> shift) & (bins - 1u) : bins;
+      const uint32_t same = __match_any_sync(0xffffffffu, d);
+      if (in && lane == (uint32_t)__ffs(same) - 1u) mine[d] += (uint16_t)__popc(same);
+      __syncwarp();
+    }
+    __syncthreads();
+    // thread t: digit t.  The warps' counts become places among this CTA's.
+    if (tid < bins) {
+      uint32_t n = 0;
+#pragma unroll 8
+      for (uint32_t w = 0; w < kClusterWarps; ++w) {
+        const uint32_t c = warp_bin[w * bins + tid];
+        warp_bin[w * bins + tid] = (uint16_t)n;
+        n += c;
+      }
+      hist[tid] = n;
+    }
+    cluster_sync();  // and all entries of the last pass have been read
+    uint32_t total = 0, before = 0;
+    if (tid < bins) {
+      for (uint32_t r = 0; r < ctas; ++r) {
+        uint32_t n;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n) : "r"(mapa_shared(&hist[tid], r)) : "memory");
+        total += n;
+        if (r < rank) before += n;
+      }
+    }
+    uint32_t sum = total;
+#pragma unroll
+    for (uint32_t o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    if (lane == 31u) warp_sum[warp] = sum;
+    __syncthreads();
+    uint32_t base = warp_sum[lane];
+#pragma unroll
+    for (uint32_t o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, base, o);
+      if (lane >= o) base += v;
+    }
+    base = __shfl_sync(0xffffffffu, base, (warp + 31u) % 32u);  // of the warps before
+    if (tid < bins) first_place[tid] = (warp ? base : 0u) + sum - total + before;
+    __syncthreads();
+    const bool last = pass + 1u == passes;
+    uint2* to = buf[pass & 1u];
+#pragma unroll
+    for (uint32_t r = 0; r < kBatch; ++r) {
+      if (r * 32u >= part) break;
+      const bool in = lo + r * 32u + lane < here;
+      const uint32_t d = in ? (e[r].x >> shift) & (bins - 1u) : bins;
+      const uint32_t same = __match_any_sync(0xffffffffu, d);
+      const uint32_t rk = __popc(same & ((1u << lane) - 1u));
+      const uint32_t place = in ? first_place[d] + mine[d] + rk : 0u;
+      __syncwarp();
+      if (in && rk == 0) mine[d] += (uint16_t)__popc(same);
+      __syncwarp();
+      if (!in) continue;
+      if (last) {
+        a.out_keys[place] = e[r].x;
+        a.out_pos[place] = e[r].y;
+      } else {
+        const uint32_t at = mapa_shared(to + (place & (chunk - 1u)), place >> chunk_log2);
+        asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(e[r].x), "r"(e[r].y) : "memory");
+      }
+    }
+    cluster_sync();  // the entries have arrived; nobody reads another's counts any more
+  }
+}
+
 // ------------------------------------------------------------------- sums
 
 struct SumArgs {
   const uint32_t* keys;
   const uint32_t* pos;
   float* parts;           // tiles x 2 x part_stride: run from the tile before, run into the tile after
+  uint32_t* runs;         // numbers of short and of long runs that cross tiles, then the tiles that they start in:
+                          // short from the front, long from the back
   uint32_t part_stride;
   uint32_t count, tiles, chunks, table_rows;
 };
@@ -274,6 +426,11 @@ __global__ void __launch_bounds__(256) sum_tiles_kernel(const tessa_lookup_grad_
       if (ends >> (b + q) & 1u) {
         const uint32_t row = __shfl_sync(0xffffffffu, key, b + q);
         const bool goes_on = b + q == 31u && next == row;
+        if (goes_on && !from_before && lane == 0 && w % s.chunks == 0) {
+          const uint64_t far = (uint64_t)first + kLongRun * kTile;
+          if (far < s.count && s.keys[far] == row) s.runs[1u + s.tiles - atomicAdd(s.runs + 1, 1u)] = tile;
+          else s.runs[2u + atomicAdd(s.runs, 1u)] = tile;
+        }
         if (in) {
           if (from_before || goes_on) {
             float* part = s.parts + ((uint64_t)tile * 2u + (from_before ? 0u : 1u)) * s.part_stride + col;
@@ -291,60 +448,74 @@ __global__ void __launch_bounds__(256) sum_tiles_kernel(const tessa_lookup_grad_
   }
 }
 
-// One block a tile: where a run starts in this tile and goes on, its parts in
-// order -- this tile's, then one of each later tile it reaches.  The threads
-// stand in rows of `groups` (4 columns each); row r adds parts r, r + R, ...,
-// and the rows' sums are added in order.
+// The runs that cross tiles, in whatever order they were noted, 128 columns at
+// a time; a run's parts are added in the order of the tiles -- the first
+// tile's, then one of each later tile it reaches.  A short run is a warp's.  Of
+// a long one warp r of a block adds parts r, r + 8, ..., and the warps' sums
+// are added in order.
 template <class O>
 __global__ void __launch_bounds__(256) sum_parts_kernel(const tessa_lookup_grad_args a, const SumArgs s) {
-  const uint32_t tile = blockIdx.x, first = tile * kTile, last = first + kTile - 1u;
-  if (last + 1u >= s.count) return;
-  const uint32_t row = s.keys[last];
-  if (row >= s.table_rows || s.keys[last + 1u] != row) return;
-  if (first && s.keys[first] == row && s.keys[first - 1u] == row) return;  // began earlier
-  uint32_t more = 0;  // later tiles that begin with the run
-  while (true) {
-    const uint64_t at = ((uint64_t)tile + 1u + more + threadIdx.x) * kTile;
-    const uint32_t got = __syncthreads_count(at < s.count && s.keys[at] == row);
-    more += got;
-    if (got < 256u) break;
-  }
+  const uint32_t pieces = (s.part_stride + 127u) / 128u;
+  const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
   __shared__ float4 sums[256];
-  const uint32_t groups = s.part_stride / 4u;
-  const uint32_t width = groups < 256u ? groups : 256u, rows = 256u / width;
-  const uint32_t r = threadIdx.x / width;
-  for (uint32_t g0 = 0; g0 < groups; g0 += width) {
-    const uint32_t g = g0 + threadIdx.x % width;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (r < rows && g < groups) {
-#pragma unroll 8
-      for (uint32_t j = r; j <= more; j += rows) {
-        const uint64_t part = j ? ((uint64_t)tile + j) * 2u : (uint64_t)tile * 2u + 1u;
-        const float4 v = *reinterpret_cast<const float4*>(s.parts + part * s.part_stride + g * 4u);
-        acc.x += v.x;
-        acc.y += v.y;
-        acc.z += v.z;
-        acc.w += v.w;
-      }
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto add = [&](const float4& v) {
+    acc.x += v.x;
+    acc.y += v.y;
+    acc.z += v.z;
+    acc.w += v.w;
+  };
+  auto part = [&](uint32_t tile, uint32_t j, uint32_t col) {
+    const uint64_t p = j ? ((uint64_t)tile + j) * 2u : (uint64_t)tile * 2u + 1u;
+    return *reinterpret_cast<const float4*>(s.parts + p * s.part_stride + col);
+  };
+  auto store = [&](uint32_t row, uint32_t col) {
+    const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      const float one[1] = {v[i]};
+      if (col + i < a.dim) store_row<O, 1>(a, row, col + i, one);
     }
-    __syncthreads();
+  };
+  const uint64_t shorts = (uint64_t)s.runs[0] * pieces, longs = (uint64_t)s.runs[1] * pieces;
+  for (uint64_t item = (uint64_t)blockIdx.x * 8u + warp; item < shorts; item += (uint64_t)gridDim.x * 8u) {
+    const uint32_t tile = s.runs[2u + item / pieces], row = s.keys[tile * kTile + kTile - 1u];
+    const uint32_t col = (uint32_t)(item % pieces) * 128u + lane * 4u;
+    // later tiles that begin with the run: at most kLongRun
+    uint32_t more = 0;
+#pragma unroll
+    for (uint32_t q = 0; q < kLongRun; q += 32u) {
+      const uint64_t at = ((uint64_t)tile + 1u + q + lane) * kTile;
+      more += __popc(__ballot_sync(0xffffffffu, at < s.count && s.keys[at] == row));
+    }
+    acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (col >= s.part_stride) continue;
+#pragma unroll 4
+    for (uint32_t j = 0; j <= more; ++j) add(part(tile, j, col));
+    store(row, col);
+  }
+  for (uint64_t item = blockIdx.x; item < longs; item += gridDim.x) {
+    const uint32_t tile = s.runs[1u + s.tiles - item / pieces], row = s.keys[tile * kTile + kTile - 1u];
+    uint32_t more = 0;
+    while (true) {
+      const uint64_t at = ((uint64_t)tile + 1u + more + threadIdx.x) * kTile;
+      const uint32_t got = __syncthreads_count(at < s.count && s.keys[at] == row);
+      more += got;
+      if (got < 256u) break;
+    }
+    const uint32_t col = (uint32_t)(item % pieces) * 128u + lane * 4u;
+    acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (col < s.part_stride) {
+#pragma unroll 8
+      for (uint32_t j = warp; j <= more; j += 8u) add(part(tile, j, col));
+    }
     sums[threadIdx.x] = acc;
     __syncthreads();
-    if (r == 0 && g < groups) {
-      for (uint32_t q = 1; q < rows; ++q) {
-        const float4 v = sums[q * width + threadIdx.x];
-        acc.x += v.x;
-        acc.y += v.y;
-        acc.z += v.z;
-        acc.w += v.w;
-      }
-      const float v[4] = {acc.x, acc.y, acc.z, acc.w};
-#pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) {
-        const float one[1] = {v[i]};
-        if (g * 4u + i < a.dim) store_row<O, 1>(a, row, g * 4u + i, one);
-      }
+    if (warp == 0 && col < s.part_stride) {
+      for (uint32_t q = 1; q < 8u; ++q) add(sums[q * 32u + lane]);
+      store(row, col);
     }
+    __syncthreads();
   }
 }
 
@@ -361,7 +532,7 @@ cudaError_t with_width(uint32_t ve, F f) {
 inline uint64_t align256(uint64_t n) { return (n + 255) / 256 * 256; }
 
 struct GradSpace {
-  uint64_t keys[2], pos[2], counts, parts, bytes;
+  uint64_t keys[2], pos[2], counts, runs, parts, bytes;
 };
 
 inline GradSpace grad_space(uint64_t count, uint64_t table_rows, uint32_t dim) {
@@ -376,6 +547,7 @@ inline GradSpace grad_space(uint64_t count, uint64_t table_rows, uint32_t dim) {
   for (int i = 0; i < 2; ++i) g.keys[i] = take(count * 4);
   for (int i = 0; i < 2; ++i) g.pos[i] = take(count * 4);
   g.counts = take((uint64_t)p.blocks * (1u << kMaxDigitBits) * 4);
+  g.runs = take((2 + div_up(count, kTile)) * 4);
   g.parts = take(div_up(count, kTile) * 2 * ((dim + 3u) / 4u * 4u) * 4);
   g.bytes = at;
   return g;
@@ -410,9 +582,11 @@ cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspa
                                   cudaStream_t stream) {
   using namespace train;
   const uint32_t eb = type_bytes(a.dtype), ob = type_bytes(a.grad_dtype);
-  if (!a.accumulate) {
-    cudaError_t e = cudaMemset2DAsync(a.grad, (a.table_rows > 1 ? a.grad_stride : a.dim) * ob, 0, (size_t)a.dim * ob,
-                                      a.table_rows, stream);
+  if (!a.accumulate) {  // the rows that no id names are zero
+    const uint64_t row_bytes = (uint64_t)a.dim * ob;
+    const cudaError_t e = a.table_rows == 1 || a.grad_stride == a.dim
+                              ? cudaMemsetAsync(a.grad, 0, a.table_rows * row_bytes, stream)
+                              : cudaMemset2DAsync(a.grad, a.grad_stride * ob, 0, row_bytes, a.table_rows, stream);
     if (e != cudaSuccess) return e;
   }
   if (a.count == 0) return cudaSuccess;
@@ -426,6 +600,7 @@ cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspa
   s.table_rows = a.table_rows;
   s.count = (uint32_t)a.count;
   s.counts = at(g.counts);
+  s.runs = at(g.runs);
   s.chunk = p.chunk;
   s.err = c.err;
   uint32_t out = 0;
@@ -433,6 +608,34 @@ cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspa
     s.out_keys = at(g.keys[0]);
     s.out_pos = at(g.pos[0]);
     sort_small_kernel<<<1, 1024, 0, stream>>>(s);
+  } else if (a.count <= kClusterMost) {
+    uint32_t chunk_log2 = 10;
+    while ((16ull << chunk_log2) < a.count) ++chunk_log2;
+    const uint32_t ctas = (uint32_t)div_up(a.count, 1ull << chunk_log2);
+    s.out_keys = at(g.keys[0]);
+    s.out_pos = at(g.pos[0]);
+    static SmemRaised raised, wide;
+    cudaError_t e = raise_smem(sort_cluster_kernel, c.device, 2 * kClusterChunk * 8 + kClusterWarps * 2 * 1024, raised);
+    const uint64_t bit = 1ull << (c.device & 63);
+    if (e == cudaSuccess && !(wide.devices.load(std::memory_order_relaxed) & bit)) {
+      e = cudaFuncSetAttribute(sort_cluster_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e == cudaSuccess) wide.devices.fetch_or(bit, std::memory_order_relaxed);
+    }
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kClusterThreads);
+    cfg.dynamicSmemBytes = (p.passes > 2 ? 2u : 1u) * (8u << chunk_log2) + (kClusterWarps * 2u << p.digit_bits);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = ctas;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, sort_cluster_kernel, s, ctas, chunk_log2, p.passes, p.digit_bits);
+    if (e != cudaSuccess) return e;
   } else {
     s.bins = 1u << p.digit_bits;
     if (s.bins < 2) s.bins = 2;
@@ -465,6 +668,7 @@ cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspa
   m.keys = at(g.keys[out]);
   m.pos = at(g.pos[out]);
   m.parts = reinterpret_cast<float*>(ws + g.parts);
+  m.runs = at(g.runs);
   m.part_stride = (a.dim + 3u) / 4u * 4u;
   m.count = (uint32_t)a.count;
   m.tiles = (uint32_t)div_up(a.count, kTile);
@@ -479,7 +683,10 @@ cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspa
     return with_type(a.grad_dtype, [&](auto o) {
       return with_width(ve, [&](auto w) {
         sum_tiles_kernel<decltype(t), decltype(o), decltype(w)::value><<<grid, 256, 0, stream>>>(a, m);
-        if (m.tiles > 1) sum_parts_kernel<decltype(o)><<<m.tiles, 256, 0, stream>>>(a, m);
+        if (m.tiles > 1) {
+          const uint64_t items = div_up((uint64_t)m.tiles * div_up(a.dim, 128), 8), most = (uint64_t)c.sm_count * 8;
+          sum_parts_kernel<decltype(o)><<<(uint32_t)(items < most ? items : most), 256, 0, stream>>>(a, m);
+        }
         return cudaGetLastError();
       });
     });
