@@ -119,7 +119,7 @@ int tessa_quantize_fp8(tessa_ctx* ctx, const tessa_fp8_quantize_args* args, void
   TRY(check_matrix("x", a.x, a.rows, a.cols, a.stride, a.dtype));
   if (a.rows > kMaxMatrix || a.cols > kMaxMatrix)
     return bad(TESSA_ERR_UNSUPPORTED, "matrix of %llu x %llu: both below 2^31", (ull)a.rows, (ull)a.cols);
-  if ((a.rows + 127) / 128 * ((a.cols + 127) / 128) > kMaxMatrix)
+  if (a.rows * ((a.cols + 127) / 128) > kMaxMatrix)
     return bad(TESSA_ERR_UNSUPPORTED, "matrix of %llu x %llu is too large", (ull)a.rows, (ull)a.cols);
   if (!a.codes != !a.scales || !a.codes_t != !a.scales_t || (!a.codes && !a.codes_t)) {
     if (a.rows && a.cols) return bad(TESSA_ERR_INVALID_ARG, "codes and scales come in pairs, one pair at least");
