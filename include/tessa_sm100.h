@@ -681,7 +681,8 @@ TESSA_API void tessa_replay_session_destroy(tessa_replay_session* session);
  * device, no scratch is kept in the context (where one is needed the caller
  * passes `workspace`, 256-byte aligned, of the size that the matching
  * *_workspace function gives; it is free again when the call's work is done),
- * and they may be captured into a CUDA graph.  What a kernel finds wrong (an
+ * and they may be captured into a CUDA graph (after a first call on the context,
+ * which sets its error word up).  What a kernel finds wrong (an
  * id outside the table: TESSA_ERR_BAD_ROW; an expired wait: TESSA_ERR_TIMEOUT)
  * is therefore reported by the next of these calls on the context, or by
  * tessa_async_status, which waits for `stream` first; either report clears it.

@@ -11,6 +11,8 @@ host side above that ABI, mirroring the reference's replay interface
 * :mod:`shear_b200.replay` -- ``TessaReplayMode``, ``TessaPreparedReplay``,
   ``prepare_tessa_replay``, ``TessaCudaReplaySession`` and
   ``run_tessa_operator_replay``;
+* :mod:`shear_b200.train` -- trains a table of vectors on the leaf operator's
+  neighbour lists: lookup, FP8 product and distillation, with their gradients;
 * :mod:`shear_b200.sharding` -- the host work queue that spreads independent
   leaf / subtree tasks over the GPUs of one box (no collective).
 

@@ -840,7 +840,7 @@ def _matrix(name: str, t, dev=None):
         raise ValueError(f"{name} is on {t.device}, not on cuda:{dev}")
     rows, cols = t.shape
     step, one = t.stride()
-    if one != 1 and cols > 1:
+    if one != 1 and cols > 1 and rows:
         raise ValueError(f"{name} must have contiguous rows (column stride 1)")
     if step < cols:
         if rows > 1:
