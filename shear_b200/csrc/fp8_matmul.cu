@@ -673,11 +673,17 @@ cudaError_t launch(const CUtensorMap& pm, const CUtensorMap& qm, const CUtensorM
 }
 
 }  // namespace mm
+
+constexpr uint64_t kFewRows = 8;
+
 }  // namespace train
+
+// Products that fp8_few_rows.cu takes.
+static bool few_rows(uint64_t m, uint64_t n) { return m <= train::kFewRows || n <= train::kFewRows; }
 
 uint64_t fp8_matmul_workspace(uint64_t m, uint64_t n, uint64_t k, int sm_count) {
   using namespace train;
-  if (m == 0 || n == 0 || k == 0) return 0;
+  if (m == 0 || n == 0 || k == 0 || few_rows(m, n)) return 0;
   const uint32_t one = mm::plan_of(m, n, k, sm_count).splits, other = mm::plan_of(n, m, k, sm_count).splits;
   const uint32_t splits = one > other ? one : other;  // which of the two depends on out's alignment
   return splits > 1 ? (uint64_t)splits * m * div_up(n, 4) * 16 : 0;
@@ -689,6 +695,7 @@ cudaError_t launch_matmul_fp8(const tessa_fp8_matmul_args& a, void* workspace, c
   const uint32_t ob = type_bytes(a.out_dtype);
   if (a.k == 0)
     return cudaMemset2DAsync(a.out, (a.m > 1 ? a.out_stride : a.n) * ob, 0, a.n * ob, a.m, stream);
+  if (few_rows(a.m, a.n)) return launch_fp8_few_rows(a, c, stream);
   // b's rows take the accumulator's lanes (then out is stored straight, 32
   // neighbours at a time) where a has few rows, which would leave the lanes
   // empty (against 200000 x 768, f32 scores: m = 16 takes 39 us so and 47

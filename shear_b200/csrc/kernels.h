@@ -248,7 +248,7 @@ struct AsyncCtx {
 int async_begin(tessa_ctx* ctx, AsyncCtx* out);
 int ctx_sm_count(const tessa_ctx* ctx);
 
-// Training operators (embedding.cu, fp8_quantize.cu, fp8_matmul.cu,
+// Training operators (embedding.cu, fp8_quantize.cu, fp8_matmul.cu, fp8_few_rows.cu,
 // distill.cu); arguments are validated by capi_train.cu.
 cudaError_t launch_embedding_lookup(const tessa_lookup_args& a, const AsyncCtx& c, cudaStream_t stream);
 uint64_t embedding_grad_workspace(uint64_t count, uint64_t table_rows, uint32_t dim);
@@ -258,6 +258,7 @@ cudaError_t launch_quantize_fp8(const tessa_fp8_quantize_args& a, const AsyncCtx
 uint64_t fp8_matmul_workspace(uint64_t m, uint64_t n, uint64_t k, int sm_count);
 cudaError_t launch_matmul_fp8(const tessa_fp8_matmul_args& a, void* workspace, const AsyncCtx& c,
                               cudaStream_t stream);
+cudaError_t launch_fp8_few_rows(const tessa_fp8_matmul_args& a, const AsyncCtx& c, cudaStream_t stream);
 uint64_t distill_workspace(uint64_t rows, uint64_t vocab, uint32_t dtype, uint32_t k, bool grad);
 cudaError_t launch_distill(const tessa_distill_args& a, void* workspace, const AsyncCtx& c, cudaStream_t stream);
 // 2-D uint8 tensor map (leaf_sq8.cu): rows x row_bytes, box of 128 bytes x

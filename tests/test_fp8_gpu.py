@@ -147,7 +147,11 @@ def _product_case(m, n, k, out, seed=0, ld=0):
     # the largest; then one rounding to the output type.
     info = torch.finfo(getattr(torch, out))
     bound = -(-pad // 32) * 33 * 2.0 ** -24 * mag + info.eps / 2 * np.abs(want)
-    err = np.abs(got.double().cpu().numpy() - want)
+    g = got.double().cpu().numpy()
+    near = np.abs(np.abs(want) - info.max) <= bound  # may round to infinity or to the largest value
+    over = (np.abs(want) > info.max) & ~near         # past what the output type holds
+    assert (g[over] == np.sign(want[over]) * np.inf).all()
+    err = np.abs(np.where(over | near, want, g) - want)
     assert (err <= bound).all(), float((err / bound).max())
     if ld:
         assert (wide[:, n:] == 5.0).all()
@@ -163,6 +167,34 @@ def _product_case(m, n, k, out, seed=0, ld=0):
 ])
 def test_product(m, n, k, out):
     _product_case(m, n, k, out)
+
+
+@pytest.mark.parametrize("m,n,k,out", [
+    (1, 5, 16, "float32"), (2, 300, 768, "bfloat16"), (3, 1000, 640, "float16"), (4, 129, 4112, "float32"),
+    (1, 20_001, 1040, "float32"), (1, 40, 16_400, "float32"), (300, 1, 400, "float32"), (1000, 3, 208, "bfloat16"),
+    (129, 4, 2048, "float32"), (4, 4, 1024, "float32"), (30_000, 2, 1296, "float16"),
+])
+def test_product_with_few_rows(m, n, k, out):
+    # one query against a table, and a table against one query
+    _product_case(m, n, k, out)
+    _product_case(m, n, k, out, seed=1, ld=5)
+
+
+@pytest.mark.parametrize("m,n", [(1, 40), (40, 2)])
+def test_few_rows_at_the_ends_of_the_scales(m, n):
+    # sixteen products of 1 * 1 under scales whose product is any power of two,
+    # past what f32 holds too; the byte 255 stands for NaN
+    import torch
+    from shear_b200 import ops
+    one = torch.full((max(m, n), 16), 0x38, dtype=torch.uint8, device="cuda")
+    for sa, sb in ((0, 0), (0, 254), (254, 0), (254, 254), (127, 127), (127, 1), (1, 1), (60, 61), (3, 104), (200, 178),
+                   (200, 183), (255, 0), (0, 255), (255, 255)):
+        a = torch.full((m, 4), sa, dtype=torch.uint8, device="cuda")
+        b = torch.full((n, 4), sb, dtype=torch.uint8, device="cuda")
+        got = ops.matmul_fp8(one[:m], a, one[:n], b).cpu().numpy()
+        with np.errstate(over="ignore", under="ignore"):
+            want = np.nan if 255 in (sa, sb) else np.float32(np.ldexp(16.0, sa + sb - 254))
+        assert np.array_equal(got, np.full((m, n), want, np.float32), equal_nan=True), (sa, sb, got.flat[0], want)
 
 
 @pytest.mark.parametrize("m,n,k", [(5, 100, 20_000), (64, 64, 40_000), (200, 768, 9000), (300, 130, 16_385)])
