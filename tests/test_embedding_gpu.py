@@ -109,8 +109,8 @@ def _zipf(rng, n, rows):
     (5, 7, 31, "float32", "float32", "int64"),
     (5, 8, 32, "bfloat16", "float32", "int64"),
     (5, 9, 33, "float16", "float16", "int32"),
-    (1000, 128, 2048, "float32", "float32", "int32"),      # the largest sort in one block
-    (1000, 128, 2049, "float32", "float32", "int32"),      # the smallest over several kernels
+    (1000, 128, 2048, "float32", "float32", "int32"),
+    (1000, 128, 2049, "float32", "float32", "int32"),
     (1023, 64, 5000, "bfloat16", "bfloat16", "int32"),     # one digit
     (1024, 64, 5000, "float32", "float32", "int64"),       # two digits
     (200_000, 128, 20_001, "float32", "float32", "int32"),
@@ -125,6 +125,17 @@ def test_grad(rows, dim, count, dtype, out, ids, zipf):
     idx = _zipf(rng, count, rows) if zipf else rng.integers(0, rows, count)
     idx[::11] = -1
     _grad_case(rows, dim, idx, dtype, out, ids, 1.25)
+
+
+@pytest.mark.parametrize("rows", [3, 900, 5000, 3_000_000])  # one to three digits
+@pytest.mark.parametrize("count", [255, 256, 257, 1024, 1025, 16_384, 16_385, 131_073])
+def test_grad_at_the_borders_of_the_sorts(rows, count):
+    # one block, one cluster of one to sixteen blocks, several kernels
+    rng = np.random.default_rng(rows + count)
+    idx = _zipf(rng, count, rows)
+    idx[5::97] = -1
+    _grad_case(rows, 4, idx, "float32", "float32", "int32", 1.0)
+    _grad_case(rows, 8, idx, "float32", "bfloat16", "int64", 1.0, accumulate=True)
 
 
 @pytest.mark.parametrize("rows,count", [(1, 5000), (2, 64), (2, 96), (3, 40_000)])
