@@ -18,10 +18,12 @@
 // One warp of a CTA stands beside the others: it reads the list, gathers the
 // listed logits, makes p and P while they read the row, and then the loss.
 //
-// Measured (B200, loss and gradient): 2048 x 16384 bf16 32.5 us (4.1 TB/s of
-// the read and the write), bound by instruction issue and the exponentials
-// (two a logit at 16 a cycle and SM: 16 us); 1024 x 1M bf16 0.96 ms (4.2 TB/s;
-// 6.4 of what the two forms together move); the loss alone 0.33 ms (6.3 TB/s).
+// Measured (B200, loss and gradient): 2048 x 16384 bf16 28 us (4.8 TB/s of the
+// read and the write), bound by instruction issue and the exponentials (two a
+// logit at 16 a cycle and SM: 16 us); 333 x 50003 f16, lists of 100, 20 us (two
+// rows an SM, so 37 of them start late; 296 rows take 12); 1024 x 1M bf16 0.96 ms
+// (4.2 TB/s; 6.4 of what the two forms together move); the loss alone 0.33 ms
+// (6.3 TB/s).
 #include "train_common.cuh"
 
 namespace tessa {
@@ -107,6 +109,10 @@ __device__ __forceinline__ uint64_t ex2_pair(uint64_t x, uint64_t neg_base, uint
 
 constexpr uint32_t kNoEntry = 0xffffffffu;
 constexpr uint32_t kListBytes = 16;        // an entry's id, p, logit and P in shared memory
+constexpr uint32_t kFilterBits = 15;       // of ids, for lists of more than a warp
+__host__ __device__ __forceinline__ uint32_t list_bytes(uint32_t k) {
+  return (k + 3u) / 4u * 4u * kListBytes + (k > 32u ? 1u << (kFilterBits - 3) : 0u);
+}
 constexpr uint32_t kSmemMost = 227u << 10;
 
 // A row's list in shared memory, k4 entries (k rounded up to four).
@@ -115,12 +121,13 @@ struct List {
   float* t;      // the teacher's logit
   float* z;      // the student's
   float* own;    // P of the id at its first entry of this CTA's slice, -1 elsewhere
+  uint32_t* filter;  // bits of ids, k > 32
   float* sums;   // maximum of t, sum of 2^((t - maximum) c): 0 if there is no entry
 };
 __device__ __forceinline__ List list_at(uint8_t* at, uint32_t k4, float* sums) {
   uint32_t* id = reinterpret_cast<uint32_t*>(at);
   float* f = reinterpret_cast<float*>(at);
-  return {id, f + k4, f + 2u * k4, f + 3u * k4, sums};
+  return {id, f + k4, f + 2u * k4, f + 3u * k4, id + 4u * k4, sums};
 }
 
 // How a row lies: its 16-byte body, and what stands before and after it (less
@@ -183,24 +190,44 @@ __device__ __forceinline__ void read_list(const tessa_distill_args& a, uint64_t 
   }
   __syncwarp();
   if (!parts) return;
+  // Nearly every id stands in a list once.  Lists of a warp are matched lane by
+  // lane; of longer ones only the entries that find their bit of the filter
+  // taken look for others, the whole warp with each (every entry with all others
+  // took 8 us for a list of 100, as long as the row itself).
+  if (a.k <= 32u) {
+    const bool in = lane < a.k && l.own[lane] >= 0.0f;
+    const uint32_t same = __match_any_sync(0xffffffffu, in ? l.id[lane] : kNoEntry);
+    if (!in) return;
+    float w = ex2((l.t[lane] - top) * c);
+    for (uint32_t more = same & ~(1u << lane); more; more &= more - 1u) w += ex2((l.t[__ffs(more) - 1] - top) * c);
+    l.own[lane] = same & ((1u << lane) - 1u) ? -1.0f : w / sum;
+    return;
+  }
+  for (uint32_t i = lane; i < 1u << (kFilterBits - 7); i += 32u) reinterpret_cast<uint4*>(l.filter)[i] = make_uint4(0, 0, 0, 0);
+  __syncwarp();
+  uint32_t taken = 0;  // bit n: entry 32 n + lane
   for (uint32_t j = lane; j < a.k; j += 32u) {
     if (l.own[j] < 0.0f) continue;
-    // Nearly every id stands in a list once: look for others without a branch.
-    const uint32_t id = l.id[j];
-    uint32_t before = 0, after = 0;
-    const uint4* ids = reinterpret_cast<const uint4*>(l.id);
-    for (uint32_t i = 0; i < k4; i += 4u) {
-      const uint4 q = ids[i / 4u];
-      const uint32_t same = (q.x == id ? 1u : 0u) | (q.y == id ? 2u : 0u) | (q.z == id ? 4u : 0u) | (q.w == id ? 8u : 0u);
-      const uint32_t low = j > i ? (j - i < 4u ? (1u << (j - i)) - 1u : 15u) : 0u;  // entries before j
-      before |= same & low;
-      after += __popc(same);
+    const uint32_t h = l.id[j] * 2654435769u >> (32u - kFilterBits);
+    if (atomicOr(l.filter + h / 32u, 1u << (h % 32u)) >> (h % 32u) & 1u) taken |= 1u << (j / 32u);
+    l.own[j] = ex2((l.t[j] - top) * c) / sum;
+  }
+  for (uint32_t n32 = 0; n32 * 32u < a.k; ++n32) {
+    for (uint32_t todo = __ballot_sync(0xffffffffu, taken >> n32 & 1u); todo; todo &= todo - 1u) {
+      const uint32_t id = l.id[n32 * 32u + __ffs(todo) - 1u];
+      uint32_t first = a.k;
+      float w = 0.0f;
+      for (uint32_t i = lane; i < a.k; i += 32u) {
+        if (l.id[i] != id) continue;
+        first = min(first, i);
+        w += ex2((l.t[i] - top) * c);
+      }
+      first = __reduce_min_sync(0xffffffffu, first);
+#pragma unroll
+      for (uint32_t o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+      for (uint32_t i = lane; i < a.k; i += 32u)
+        if (l.id[i] == id) l.own[i] = i == first ? w / sum : -1.0f;
     }
-    float w = ex2((l.t[j] - top) * c);
-    if (after > 1u && before == 0u)  // the first of several
-      for (uint32_t i = j + 1u; i < a.k; ++i)
-        if (l.id[i] == id) w += ex2((l.t[i] - top) * c);
-    l.own[j] = before ? -1.0f : w / sum;
   }
 }
 
@@ -303,7 +330,7 @@ struct DistillPlan {
 };
 
 template <class T, int WARPS>
-__global__ void __launch_bounds__((WARPS + 1) * 32)
+__global__ void __launch_bounds__((WARPS + 1) * 32, WARPS == 16 ? 2 : WARPS == 8 ? 5 : 9)
     distill_kernel(const tessa_distill_args a, const DistillPlan plan, uint32_t* err) {
   constexpr uint32_t VE = 16u / sizeof(T), NT = WARPS * 32u;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -312,7 +339,7 @@ __global__ void __launch_bounds__((WARPS + 1) * 32)
   __shared__ Stat warp_stat[WARPS];
   __shared__ Stat cta_stat[16];
   const List l = list_at(smem, k4, sums);
-  uint4* kept = reinterpret_cast<uint4*>(smem + k4 * kListBytes);
+  uint4* kept = reinterpret_cast<uint4*>(smem + list_bytes(a.k));
 
   const uint32_t tid = threadIdx.x, warp = tid / 32u, lane = tid % 32u;
   const uint32_t C = 1u << plan.cluster_log2, rank = blockIdx.x & (C - 1u);
@@ -477,7 +504,7 @@ cudaError_t launch_cluster(const tessa_distill_args& a, const DistillPlan& plan,
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((uint32_t)(a.rows << plan.cluster_log2));
   cfg.blockDim = dim3((WARPS + 1) * 32);
-  cfg.dynamicSmemBytes = (a.k + 3u) / 4u * 4u * kListBytes + plan.keep_bytes;
+  cfg.dynamicSmemBytes = list_bytes(a.k) + plan.keep_bytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -508,7 +535,7 @@ cudaError_t launch_distill(const tessa_distill_args& a, void* workspace, const A
   const bool apart = distill_workspace(a.rows, a.vocab, a.dtype, a.k, a.grad != nullptr) != 0;
   DistillPlan plan = {};
   // The fewest CTAs a row that can keep it (a cluster costs: 2048 x 16384 bf16
-  // takes 33 us with one CTA a row, 47 with two), more while rows alone do not
+  // takes 28 us with one CTA a row, 39 with two), more while rows alone do not
   // fill the GPU.
   while (plan.cluster_log2 < 3 &&
          ((a.grad && !apart && bytes >> plan.cluster_log2 > kKeep) ||

@@ -150,6 +150,21 @@ def test_masks_and_short_lists(dtype, vocab, rows, tau):
     _check(z.double().numpy(), i, t.astype(np.float64), tau, w, dtype, got)
 
 
+@pytest.mark.parametrize("k", [31, 32, 33, 100, 1024])
+@pytest.mark.parametrize("pool", [1, 7, 300, 5000])
+@pytest.mark.parametrize("vocab", [5003, 120_001])
+def test_repeated_ids(k, pool, vocab):
+    # lists of a warp and longer ones, with few, some and nearly no ids twice;
+    # rows of one CTA, and rows that a cluster shares
+    rng = np.random.default_rng(k + pool)
+    z, _, t = _make(rng, 6, vocab, 4, "float32")
+    t = (rng.standard_normal((6, k)) * 3).astype(np.float32)
+    i = rng.permutation(vocab)[:pool][rng.integers(0, pool, (6, k))]
+    i[3, ::3] = -1
+    got = _run(z, i, t, 1.5, None)
+    _check(z.double().numpy(), i, t.astype(np.float64), 1.5, np.ones(6), "float32", got)
+
+
 def test_nan_and_inf_stay_in_their_row():
     import torch
     from shear_b200 import ops
