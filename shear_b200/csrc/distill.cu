@@ -553,9 +553,12 @@ cudaError_t launch_distill(const tessa_distill_args& a, void* workspace, const A
   }
   return with_type(a.dtype, [&](auto t) {
     using T = decltype(t);
-    // short rows leave more warps idle than they occupy: 8192 x 2000 f32 takes
-    // 43 us with four warps, 56 with eight
-    const uint32_t w = slice <= 16384 ? 4 : slice <= 65536 ? 8 : 16;
+    // Short rows leave more warps idle than they occupy: 8192 x 2000 f32 takes
+    // 43 us with four warps, 56 with eight.  Where shared memory lets two CTAs
+    // stand on an SM, they have 16 each; the loss alone keeps nothing (4096 x
+    // 50000 bf16: 70 us with eight, 93 with 16), until rows are so long that a
+    // CTA's end no longer counts (1024 x 1M bf16: 347 us with eight, 322 with 16).
+    const uint32_t w = slice <= 16384 ? 4 : slice <= 65536 || (!plan.keep_bytes && slice < kApart) ? 8 : 16;
     cudaError_t e = w == 4   ? launch_cluster<T, 4>(first, plan, c, stream)
                     : w == 8 ? launch_cluster<T, 8>(first, plan, c, stream)
                              : launch_cluster<T, 16>(first, plan, c, stream);
