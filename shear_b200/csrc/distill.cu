@@ -18,12 +18,12 @@
 // One warp of a CTA stands beside the others: it reads the list, gathers the
 // listed logits, makes p and P while they read the row, and then the loss.
 //
-// Measured (B200, loss and gradient): 2048 x 16384 bf16 28 us (4.8 TB/s of the
-// read and the write), bound by instruction issue and the exponentials (two a
-// logit at 16 a cycle and SM: 16 us); 333 x 50003 f16, lists of 100, 20 us (two
-// rows an SM, so 37 of them start late; 296 rows take 12); 1024 x 1M bf16 0.96 ms
-// (4.2 TB/s; 6.4 of what the two forms together move); the loss alone 0.33 ms
-// (6.3 TB/s).
+// Measured (B200, loss and gradient, rows from DRAM): 2048 x 16384 bf16 28 us
+// (4.8 TB/s of the read and the write), bound by instruction issue and the
+// exponentials (two a logit at 16 a cycle and SM: 16 us); 4096 x 50000 bf16 177
+// us (4.6 TB/s); 296 x 50003 f16 16 us, but 333 rows 24: two rows an SM, so 37
+// of them start late; 1024 x 1M bf16 0.95 ms (4.3 TB/s; 6.4 of what the two forms
+// together move); the loss alone 0.32 ms (6.4 TB/s).
 #include "train_common.cuh"
 
 namespace tessa {
@@ -156,27 +156,50 @@ __device__ __forceinline__ void read_list(const tessa_distill_args& a, uint64_t 
   constexpr uint32_t VE = 16u / sizeof(T);
   const uint32_t k4 = (a.k + 3u) / 4u * 4u;
   float top = -INFINITY;
-  for (uint32_t j = lane; j < k4; j += 32u) {
-    uint32_t id = kNoEntry;
-    float t = -INFINITY;
-    if (j < a.k) {
-      const uint64_t at = row * a.k + j;
-      const int64_t v = a.id_bits == 32 ? (int64_t)static_cast<const int32_t*>(a.teacher_ids)[at]
-                                        : static_cast<const int64_t*>(a.teacher_ids)[at];
-      t = a.teacher_logits[at];
-      if (v >= 0 && (uint64_t)v < a.vocab) {
-        if (t != -INFINITY) id = (uint32_t)v;
-      } else if (v != -1) {
-        report(err, TESSA_DEVERR_BAD_ROW);
+  // N entries a lane at a time: their reads are under way together, and then the listed logits'.
+  auto read = [&](auto count) {
+    constexpr uint32_t N = decltype(count)::value;
+    for (uint32_t j0 = lane; j0 < k4; j0 += 32u * N) {
+      int64_t v[N];
+      float t[N], x[N];
+#pragma unroll
+      for (uint32_t u = 0; u < N; ++u) {
+        const uint32_t j = j0 + u * 32u;
+        const uint64_t at = row * a.k + j;
+        v[u] = -1;
+        t[u] = -INFINITY;
+        if (j < a.k) {
+          v[u] = a.id_bits == 32 ? (int64_t)static_cast<const int32_t*>(a.teacher_ids)[at]
+                                 : static_cast<const int64_t*>(a.teacher_ids)[at];
+          t[u] = a.teacher_logits[at];
+        }
+      }
+      uint32_t id[N], mine = 0;
+#pragma unroll
+      for (uint32_t u = 0; u < N; ++u) {
+        const bool in = v[u] >= 0 && (uint64_t)v[u] < a.vocab;
+        if (!in && v[u] != -1) report(err, TESSA_DEVERR_BAD_ROW);
+        id[u] = in && t[u] != -INFINITY ? (uint32_t)v[u] : kNoEntry;
+        if (id[u] != kNoEntry && (id[u] < s.head || id[u] >= s.tail0 ? ends : (id[u] - s.head) / VE - lo < n)) mine |= 1u << u;
+        x[u] = mine >> u & 1u || (every && id[u] != kNoEntry) ? to_f32(z[id[u]]) : 0.0f;
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < N; ++u) {
+        const uint32_t j = j0 + u * 32u;
+        if (j >= k4) break;
+        l.id[j] = id[u];
+        l.t[j] = t[u];
+        l.z[j] = x[u];
+        l.own[j] = mine >> u & 1u ? 0.0f : -1.0f;
+        if (id[u] != kNoEntry) top = fmaxf(top, t[u]);
       }
     }
-    l.id[j] = id;
-    l.t[j] = t;
-    if (id != kNoEntry) top = fmaxf(top, t);
-    const bool mine = id != kNoEntry && (id < s.head || id >= s.tail0 ? ends : (id - s.head) / VE - lo < n);
-    l.z[j] = (mine || (every && id != kNoEntry)) ? to_f32(z[id]) : 0.0f;
-    l.own[j] = mine ? 0.0f : -1.0f;
-  }
+  };
+  // (with lists of 32 four at a time cost issue slots: 2048 x 16384 bf16 32 us
+  // instead of 28; with lists of 100 one at a time: 333 x 50003
+  // f16 29 us instead of 27)
+  if (a.k <= 32u) read(std::integral_constant<int, 1>());
+  else read(std::integral_constant<int, 4>());
 #pragma unroll
   for (uint32_t o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   float sum = 0.0f;
