@@ -11,10 +11,9 @@
 // run that crosses a tile border leaves its part in the workspace, and a last
 // kernel adds each such run's parts.  Every tile holds 32 entries however
 // popular one id is, so skew costs nothing but the parts.  131072 rows of 128
-// f32 into 200000: 70 us, of which clearing 17, the sort 24 (latency), the tiles
-// 17 (4 TB/s), parts 9; adding to the gradient instead 52.  Clearing the rows
-// that no id names on a second stream, beside the sort, gained nothing
-// (200000 x 128 f32 88 us either way, 1M x 768 bf16 428): it is in order.
+// f32 into 200000: 67 us, of which the sort 24 (latency; the rows that no id
+// names are cleared beside it), the tiles 17 (4 TB/s), parts 9; adding to the
+// gradient instead 51.
 #include "train_common.cuh"
 
 namespace tessa {
@@ -94,8 +93,19 @@ struct SortArgs {
   uint32_t* runs;         // two counters, cleared for the sums
   uint64_t table_rows;
   uint32_t count, chunk, shift, bins;
+  uint32_t blocks;        // that sort; those behind them clear
+  uint4* clear;
+  uint64_t clear_count;
   uint32_t* err;
 };
+
+// A block behind the sort's: its share of the gradient's memory becomes zero.
+__device__ __forceinline__ void clear_share(const SortArgs& a) {
+  const uint64_t step = (uint64_t)(gridDim.x - a.blocks) * blockDim.x;
+#pragma unroll 8
+  for (uint64_t i = (uint64_t)(blockIdx.x - a.blocks) * blockDim.x + threadIdx.x; i < a.clear_count; i += step)
+    a.clear[i] = make_uint4(0u, 0u, 0u, 0u);
+}
 
 template <bool FIRST>
 __device__ __forceinline__ uint32_t sort_key(const SortArgs& a, uint32_t i, uint32_t* err) {
@@ -105,6 +115,7 @@ __device__ __forceinline__ uint32_t sort_key(const SortArgs& a, uint32_t i, uint
 template <bool FIRST>
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const SortArgs a) {
   __shared__ uint32_t bin[1u << kMaxDigitBits];
+  if (blockIdx.x >= a.blocks) return clear_share(a);
   for (uint32_t b = threadIdx.x; b < a.bins; b += kSortThreads) bin[b] = 0;
   __syncthreads();
   const uint32_t lo = blockIdx.x * a.chunk, hi = min(a.count, lo + a.chunk);
@@ -128,6 +139,7 @@ template <bool FIRST>
 __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortArgs a) {
   extern __shared__ __align__(16) uint32_t warp_bin[];  // kSortWarps x bins: counts, then next places
   __shared__ uint32_t warp_sum[kSortWarps];
+  if (blockIdx.x >= a.blocks) return clear_share(a);
   const uint32_t tid = threadIdx.x, warp = tid / 32u, lane = tid % 32u;
   const uint32_t part = a.chunk / kSortWarps;  // a multiple of 32
   const uint32_t lo = min(a.count, blockIdx.x * a.chunk + warp * part), hi = min(a.count, lo + part);
@@ -150,7 +162,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortAr
   if (2u * tid < a.bins) {
     const uint2* c = reinterpret_cast<const uint2*>(a.counts) + tid;
 #pragma unroll 8
-    for (uint32_t b = 0; b < gridDim.x; ++b) {
+    for (uint32_t b = 0; b < a.blocks; ++b) {
       const uint2 n = c[(uint64_t)b * (a.bins / 2u)];
       if (b < blockIdx.x) {
         before[0] += n.x;
@@ -227,6 +239,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortAr
 constexpr uint32_t kSmallThreads = kSmallSort / 2;
 __global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(const SortArgs a) {
   __shared__ uint64_t e[kSmallSort];
+  if (blockIdx.x >= a.blocks) return clear_share(a);
   if (threadIdx.x < 2u) a.runs[threadIdx.x] = 0u;
   uint32_t n = 32;
   while (n < a.count) n <<= 1;
@@ -263,12 +276,13 @@ constexpr uint32_t kClusterChunk = 1024, kClusterWarps = kClusterChunk / 32;
 constexpr uint32_t kClusterMost = 16u * kClusterChunk;
 
 __global__ void __launch_bounds__(kClusterChunk)
-    sort_cluster_kernel(const SortArgs a, uint32_t ctas, uint32_t passes, uint32_t digit_bits) {
+    sort_cluster_kernel(const SortArgs a, uint32_t passes, uint32_t digit_bits) {
   extern __shared__ uint16_t warp_digits[];  // warps x bins
   __shared__ uint2 entry[2][kClusterChunk];
   __shared__ uint32_t hist[1u << kMaxDigitBits], first_place[1u << kMaxDigitBits];
   __shared__ uint32_t warp_sum[kClusterWarps];
-  const uint32_t bins = 1u << digit_bits;
+  if (blockIdx.x >= a.blocks) return clear_share(a);  // whole clusters
+  const uint32_t ctas = a.blocks, bins = 1u << digit_bits;
   const uint32_t tid = threadIdx.x, warp = tid / 32u, lane = tid % 32u, rank = cluster_ctarank();
   const uint32_t at = rank * kClusterChunk + tid;
   uint16_t* mine = warp_digits + warp * bins;
@@ -523,6 +537,8 @@ cudaError_t with_width(uint32_t ve, F f) {
 
 inline uint64_t align256(uint64_t n) { return (n + 255) / 256 * 256; }
 
+constexpr uint64_t kBeside = 100ull << 20;  // bytes of a gradient that is cleared beside the sort
+
 struct GradSpace {
   uint64_t keys[2], pos[2], counts, runs, parts, bytes;
 };
@@ -567,18 +583,25 @@ cudaError_t launch_embedding_lookup(const tessa_lookup_args& a, const AsyncCtx& 
 }
 
 uint64_t embedding_grad_workspace(uint64_t count, uint64_t table_rows, uint32_t dim) {
-  return train::grad_space(count, table_rows, dim).bytes;
+  return count ? train::grad_space(count, table_rows, dim).bytes : 0;
 }
 
 cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspace, const AsyncCtx& c,
                                   cudaStream_t stream) {
   using namespace train;
   const uint32_t eb = type_bytes(a.dtype), ob = type_bytes(a.grad_dtype);
-  if (!a.accumulate) {  // the rows that no id names are zero
-    const uint64_t row_bytes = (uint64_t)a.dim * ob;
-    const cudaError_t e = a.table_rows == 1 || a.grad_stride == a.dim
-                              ? cudaMemsetAsync(a.grad, 0, a.table_rows * row_bytes, stream)
-                              : cudaMemset2DAsync(a.grad, a.grad_stride * ob, 0, row_bytes, a.table_rows, stream);
+  // The rows that no id names are zero.  Where stores at a kernel's rate are
+  // through before the sort, which leaves most SMs idle, blocks beside it clear
+  // them (200000 rows, 16384 ids: 64 columns of bf16 25 us instead of 29, 128 of
+  // f32 39 instead of 43; 120000 x 256 f32, 117 MB, 46 either way).  A larger
+  // gradient is cleared first, at the memory's rate.
+  const uint64_t row_bytes = (uint64_t)a.dim * ob, bytes = a.table_rows * row_bytes;
+  const bool whole = a.table_rows == 1 || a.grad_stride == a.dim;
+  const bool beside = !a.accumulate && a.count > 0 && whole && bytes <= kBeside && bytes % 16 == 0 &&
+                      reinterpret_cast<uintptr_t>(a.grad) % 16 == 0;
+  if (!a.accumulate && !beside) {
+    const cudaError_t e = whole ? cudaMemsetAsync(a.grad, 0, bytes, stream)
+                                : cudaMemset2DAsync(a.grad, a.grad_stride * ob, 0, row_bytes, a.table_rows, stream);
     if (e != cudaSuccess) return e;
   }
   if (a.count == 0) return cudaSuccess;
@@ -595,11 +618,23 @@ cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspa
   s.runs = at(g.runs);
   s.chunk = p.chunk;
   s.err = c.err;
+  s.clear = static_cast<uint4*>(a.grad);
+  // blocks for this launch's share, of `launches`
+  auto share = [&](uint32_t launch, uint32_t launches) {
+    if (!beside) return 0u;
+    const uint64_t all = bytes / 16, lo = all * launch / launches, hi = all * (launch + 1) / launches;
+    s.clear = static_cast<uint4*>(a.grad) + lo;
+    s.clear_count = hi - lo;
+    const uint64_t want = div_up(s.clear_count, 4096);
+    return (uint32_t)(want < (uint64_t)c.sm_count ? want : (uint64_t)c.sm_count);
+  };
   uint32_t out = 0;
   if (a.count <= kSmallSort) {
     s.out_keys = at(g.keys[0]);
     s.out_pos = at(g.pos[0]);
-    sort_small_kernel<<<1, kSmallThreads, 0, stream>>>(s);
+    s.blocks = 1;
+    const uint32_t extra = share(0, 1) * 4u;
+    sort_small_kernel<<<1 + extra, kSmallThreads, 0, stream>>>(s);
   } else if (a.count <= kClusterMost) {
     const uint32_t ctas = (uint32_t)div_up(a.count, kClusterChunk);
     s.out_keys = at(g.keys[0]);
@@ -613,7 +648,9 @@ cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspa
     }
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas);
+    s.blocks = ctas;
+    cfg.gridDim = dim3(ctas + share(0, 1) / ctas * ctas);
+    if (beside && cfg.gridDim.x == ctas) cfg.gridDim.x += ctas;
     cfg.blockDim = dim3(kClusterChunk);
     cfg.dynamicSmemBytes = kClusterWarps * 2u << p.digit_bits;
     cfg.stream = stream;
@@ -624,9 +661,10 @@ cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspa
     attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, sort_cluster_kernel, s, ctas, p.passes, p.digit_bits);
+    e = cudaLaunchKernelEx(&cfg, sort_cluster_kernel, s, p.passes, p.digit_bits);
     if (e != cudaSuccess) return e;
   } else {
+    s.blocks = p.blocks;
     s.bins = 1u << p.digit_bits;
     if (s.bins < 2) s.bins = 2;
     const uint32_t smem = kSortWarps * s.bins * 4u;
@@ -642,13 +680,12 @@ cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspa
       s.out_keys = at(g.keys[out]);
       s.out_pos = at(g.pos[out]);
       s.shift = pass * p.digit_bits;
-      if (pass == 0) {
-        sort_count_kernel<true><<<p.blocks, kSortThreads, 0, stream>>>(s);
-        sort_scatter_kernel<true><<<p.blocks, kSortThreads, smem, stream>>>(s);
-      } else {
-        sort_count_kernel<false><<<p.blocks, kSortThreads, 0, stream>>>(s);
-        sort_scatter_kernel<false><<<p.blocks, kSortThreads, smem, stream>>>(s);
-      }
+      const uint32_t launches = 2 * p.passes, count_blocks = p.blocks + share(2 * pass, launches);
+      if (pass == 0) sort_count_kernel<true><<<count_blocks, kSortThreads, 0, stream>>>(s);
+      else sort_count_kernel<false><<<count_blocks, kSortThreads, 0, stream>>>(s);
+      const uint32_t scatter_blocks = p.blocks + share(2 * pass + 1, launches);
+      if (pass == 0) sort_scatter_kernel<true><<<scatter_blocks, kSortThreads, smem, stream>>>(s);
+      else sort_scatter_kernel<false><<<scatter_blocks, kSortThreads, smem, stream>>>(s);
     }
   }
   cudaError_t e = cudaGetLastError();
