@@ -52,7 +52,9 @@ constexpr uint32_t kSortWarps = kSortThreads / 32;
 constexpr uint32_t kMaxDigitBits = 10;
 constexpr uint32_t kBatch = 8;         // keys a thread has under way
 constexpr uint32_t kSmallSort = 256;   // entries that one block sorts by comparison
-constexpr uint32_t kTile = 32;         // sorted entries a warp sums
+constexpr uint32_t kTile = 32;         // sorted entries a warp sums,
+constexpr uint32_t kShortTile = 8;     // and where there are few: a warp's chain of reads is what they wait for
+constexpr uint64_t kFewIds = 8192;      // (4096 of 128 f32 17 us, 19 with long tiles; 16384 x 768 bf16 31 and 27)
 constexpr uint32_t kLongRun = 64;      // tiles that a run goes on for, from which a block adds its parts
 
 struct SortPlan {
@@ -359,7 +361,7 @@ struct SumArgs {
   uint32_t* runs;         // numbers of short and of long runs that cross tiles, then the tiles that they start in:
                           // short from the front, long from the back
   uint32_t part_stride;
-  uint32_t count, tiles, chunks, table_rows;
+  uint32_t count, tile, tiles, chunks, table_rows;  // tile: entries of one
 };
 
 template <class O, int VE>
@@ -377,23 +379,24 @@ __device__ __forceinline__ void store_row(const tessa_lookup_grad_args& a, uint3
   *grad_at<O, VE>(a, row, c) = o;
 }
 
-// One warp: the 32 sorted entries of a tile, 32 * VE columns.
-template <class T, class O, int VE, bool ACC>
+// One warp: the TILE sorted entries of a tile, 32 * VE columns.
+template <class T, class O, int VE, bool ACC, uint32_t TILE>
 __global__ void __launch_bounds__(256) sum_tiles_kernel(const tessa_lookup_grad_args a, const SumArgs s) {
   const uint64_t w = (uint64_t)blockIdx.x * 8u + threadIdx.x / 32u;
   const uint32_t tile = (uint32_t)(w / s.chunks), lane = threadIdx.x % 32u;
   if (tile >= s.tiles) return;
   const uint32_t col = (uint32_t)(w % s.chunks) * 32u * VE + lane * VE;
   const bool in = col < a.dim;
-  const uint32_t first = tile * kTile, e = first + lane;
-  const uint32_t key = e < s.count ? s.keys[e] : s.table_rows;
-  const uint32_t pos = e < s.count ? s.pos[e] : 0u;
+  const uint32_t first = tile * TILE, e = first + lane;
+  const bool here = lane < TILE && e < s.count;
+  const uint32_t key = here ? s.keys[e] : s.table_rows;
+  const uint32_t pos = here ? s.pos[e] : 0u;
   const uint32_t valid = __popc(__ballot_sync(0xffffffffu, key < s.table_rows));  // padding is sorted last
   if (valid == 0) return;
   const uint32_t prev = first ? s.keys[first - 1u] : s.table_rows;
-  const uint32_t next = first + kTile < s.count ? s.keys[first + kTile] : s.table_rows;
+  const uint32_t next = first + TILE < s.count ? s.keys[first + TILE] : s.table_rows;
   const uint32_t after = __shfl_down_sync(0xffffffffu, key, 1);
-  const uint32_t ends = __ballot_sync(0xffffffffu, lane == 31u || after != key);
+  const uint32_t ends = __ballot_sync(0xffffffffu, lane == TILE - 1u || after != key);
   const T* dout = static_cast<const T*>(a.dout) + col;
   float acc[VE];
 #pragma unroll
@@ -423,9 +426,9 @@ __global__ void __launch_bounds__(256) sum_tiles_kernel(const tessa_lookup_grad_
       for (int i = 0; i < VE; ++i) acc[i] += to_f32(x[q].v[i]);
       if (ends >> (b + q) & 1u) {
         const uint32_t row = __shfl_sync(0xffffffffu, key, b + q);
-        const bool goes_on = b + q == 31u && next == row;
+        const bool goes_on = b + q == TILE - 1u && next == row;
         if (goes_on && !from_before && lane == 0 && w % s.chunks == 0) {
-          const uint64_t far = (uint64_t)first + kLongRun * kTile;
+          const uint64_t far = (uint64_t)first + kLongRun * TILE;
           if (far < s.count && s.keys[far] == row) s.runs[1u + s.tiles - atomicAdd(s.runs + 1, 1u)] = tile;
           else s.runs[2u + atomicAdd(s.runs, 1u)] = tile;
         }
@@ -483,14 +486,14 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(const tessa_lookup_grad_
   };
   const uint64_t shorts = (uint64_t)s.runs[0] * pieces, longs = (uint64_t)s.runs[1] * pieces;
   for (uint64_t item = (uint64_t)blockIdx.x * 8u + warp; item < shorts; item += (uint64_t)gridDim.x * 8u) {
-    const uint32_t tile = s.runs[2u + item / pieces], row = s.keys[tile * kTile + kTile - 1u];
+    const uint32_t tile = s.runs[2u + item / pieces], row = s.keys[(tile + 1u) * s.tile - 1u];
     const uint32_t col = (uint32_t)(item % pieces) * 128u + lane * 4u;
     load_old(row, col);
     // later tiles that begin with the run: at most kLongRun
     uint32_t more = 0;
 #pragma unroll
     for (uint32_t q = 0; q < kLongRun; q += 32u) {
-      const uint64_t at = ((uint64_t)tile + 1u + q + lane) * kTile;
+      const uint64_t at = ((uint64_t)tile + 1u + q + lane) * s.tile;
       more += __popc(__ballot_sync(0xffffffffu, at < s.count && s.keys[at] == row));
     }
     acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -500,10 +503,10 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(const tessa_lookup_grad_
     store(row, col);
   }
   for (uint64_t item = blockIdx.x; item < longs; item += gridDim.x) {
-    const uint32_t tile = s.runs[1u + s.tiles - item / pieces], row = s.keys[tile * kTile + kTile - 1u];
+    const uint32_t tile = s.runs[1u + s.tiles - item / pieces], row = s.keys[(tile + 1u) * s.tile - 1u];
     uint32_t more = 0;
     while (true) {
-      const uint64_t at = ((uint64_t)tile + 1u + more + threadIdx.x) * kTile;
+      const uint64_t at = ((uint64_t)tile + 1u + more + threadIdx.x) * s.tile;
       const uint32_t got = __syncthreads_count(at < s.count && s.keys[at] == row);
       more += got;
       if (got < 256u) break;
@@ -555,8 +558,9 @@ inline GradSpace grad_space(uint64_t count, uint64_t table_rows, uint32_t dim) {
   for (int i = 0; i < 2; ++i) g.keys[i] = take(count * 4);
   for (int i = 0; i < 2; ++i) g.pos[i] = take(count * 4);
   g.counts = take((uint64_t)p.blocks * (1u << kMaxDigitBits) * 4);
-  g.runs = take((2 + div_up(count, kTile)) * 4);
-  g.parts = take(div_up(count, kTile) * 2 * ((dim + 3u) / 4u * 4u) * 4);
+  const uint64_t tiles = div_up(count, count <= kFewIds ? kShortTile : kTile);
+  g.runs = take((2 + tiles) * 4);
+  g.parts = take(tiles * 2 * ((dim + 3u) / 4u * 4u) * 4);
   g.bytes = at;
   return g;
 }
@@ -698,7 +702,8 @@ cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspa
   m.runs = at(g.runs);
   m.part_stride = (a.dim + 3u) / 4u * 4u;
   m.count = (uint32_t)a.count;
-  m.tiles = (uint32_t)div_up(a.count, kTile);
+  m.tile = a.count <= kFewIds ? kShortTile : kTile;
+  m.tiles = (uint32_t)div_up(a.count, m.tile);
   m.table_rows = (uint32_t)a.table_rows;
   const uint32_t most = 16u / (eb > ob ? eb : ob);
   uint32_t ve = vector_elems(a.dout, a.count, a.dim, a.dout_stride, eb, most);
@@ -710,8 +715,16 @@ cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspa
     return with_type(a.grad_dtype, [&](auto o) {
       return with_width(ve, [&](auto w) {
         constexpr int VE = decltype(w)::value;
-        if (a.accumulate) sum_tiles_kernel<decltype(t), decltype(o), VE, true><<<grid, 256, 0, stream>>>(a, m);
-        else sum_tiles_kernel<decltype(t), decltype(o), VE, false><<<grid, 256, 0, stream>>>(a, m);
+        auto tiles = [&](auto tile, auto add) {
+          sum_tiles_kernel<decltype(t), decltype(o), VE, decltype(add)::value, decltype(tile)::value>
+              <<<grid, 256, 0, stream>>>(a, m);
+        };
+        auto either = [&](auto tile) {
+          if (a.accumulate) tiles(tile, std::true_type());
+          else tiles(tile, std::false_type());
+        };
+        if (m.tile == kTile) either(std::integral_constant<uint32_t, kTile>());
+        else either(std::integral_constant<uint32_t, kShortTile>());
         if (m.tiles > 1) {
           const uint64_t items = div_up((uint64_t)m.tiles * div_up(a.dim, 128), 8), most = (uint64_t)c.sm_count * 8;
           const uint32_t blocks = (uint32_t)(items < most ? items : most);
