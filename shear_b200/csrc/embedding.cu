@@ -5,7 +5,8 @@
 //
 // Gradient: grad[v] = s * sum_{t: id_t = v} dout[t].  Atomic adds would give
 // another order, and other bits, every time, and a popular row would serialise
-// them.  Here the entries (id, t) are sorted (stable radix sort, digits of at
+// them.  A few thousand entries are compared with one another (below); more
+// (id, t) are sorted (stable radix sort, digits of at
 // most 10 bits), cut into tiles of 32 sorted entries, and one warp sums a
 // tile's rows run by run in f32: a run inside the tile is written at once, a
 // run that crosses a tile border leaves its part in the workspace, and a last
@@ -51,7 +52,13 @@ constexpr uint32_t kSortThreads = 512;
 constexpr uint32_t kSortWarps = kSortThreads / 32;
 constexpr uint32_t kMaxDigitBits = 10;
 constexpr uint32_t kBatch = 8;         // keys a thread has under way
-constexpr uint32_t kSmallSort = 256;   // entries that one block sorts by comparison
+
+// Entries that are compared instead of sorted: 4096, and fewer or none of wide
+// rows, because one block has all rows of an id and one warp all columns (skewed
+// ids; 1024 over 20000 x 128 f32 7 us, 15 sorted; 4096 17 either way; 1024 x 768
+// bf16 13 and 17; 2048 x 768 19 and 18; 256 x 2048 f32 55 and 36).
+inline bool unsorted(uint64_t count, uint32_t dim) { return count <= 4096 && dim <= 768 && count * dim <= 1u << 20; }
+
 constexpr uint32_t kTile = 32;         // sorted entries a warp sums,
 constexpr uint32_t kShortTile = 8;     // and where there are few: a warp's chain of reads is what they wait for
 constexpr uint64_t kFewIds = 8192;      // (4096 of 128 f32 17 us, 19 with long tiles; 16384 x 768 bf16 31 and 27)
@@ -233,37 +240,6 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortAr
         a.out_pos[place] = pos[r];
       }
     }
-  }
-}
-
-// Few entries: one block, a bitonic sort of (key, position) in shared memory (16
-// entries: 2.5 us less than the cluster's sort below; from 512 on it is slower).
-constexpr uint32_t kSmallThreads = kSmallSort / 2;
-__global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(const SortArgs a) {
-  __shared__ uint64_t e[kSmallSort];
-  if (blockIdx.x >= a.blocks) return clear_share(a);
-  if (threadIdx.x < 2u) a.runs[threadIdx.x] = 0u;
-  uint32_t n = 32;
-  while (n < a.count) n <<= 1;
-  for (uint32_t i = threadIdx.x; i < n; i += kSmallThreads)
-    e[i] = i < a.count ? (uint64_t)id_key(a.ids, a.id_bits, i, a.table_rows, a.err) << 32 | i : ~0ull;
-  for (uint32_t size = 2; size <= n; size <<= 1) {
-    for (uint32_t step = size >> 1; step; step >>= 1) {
-      __syncthreads();
-      for (uint32_t j = threadIdx.x; j < n / 2; j += kSmallThreads) {
-        const uint32_t lo = 2u * j - (j & (step - 1u)), hi = lo + step;
-        const uint64_t x = e[lo], y = e[hi];
-        if ((x > y) == ((lo & size) == 0u)) {
-          e[lo] = y;
-          e[hi] = x;
-        }
-      }
-    }
-  }
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i < a.count; i += kSmallThreads) {
-    a.out_keys[i] = (uint32_t)(e[i] >> 32);
-    a.out_pos[i] = (uint32_t)e[i];
   }
 }
 
@@ -528,6 +504,165 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(const tessa_lookup_grad_
   }
 }
 
+// ------------------------------------------------------ few ids, one launch
+
+// Up to 4096 entries: a block keeps all keys in shared memory, and a warp
+// has one entry.  If no earlier one has its key, the warp sums the rows of all
+// that have, in order; more than 32 of them are shared by the block's warps,
+// each a part of the entries, whose sums are added in order.  Blocks behind
+// these clear the rows that no id names, which they mark in a bitmap, so one
+// launch does it all: 256 ids over 20000 x 128 f32 4.2 us, by sorting 11.5; over
+// 200000 19 and 23, mostly clearing.  Bound by
+// the latency of three dependent reads, and by an id's rows where it has many.
+constexpr uint32_t kFewWarps = 8;
+
+template <class T, class O, int VE, bool ACC>
+__global__ void __launch_bounds__(256) few_ids_kernel(const tessa_lookup_grad_args a, uint32_t sum_blocks, uint32_t* err) {
+  extern __shared__ __align__(16) uint32_t few_smem[];
+  const uint32_t tid = threadIdx.x, warp = tid / 32u, lane = tid % 32u, count = (uint32_t)a.count;
+  const uint32_t none = (uint32_t)a.table_rows;
+  auto key_of = [&](uint32_t i) {
+    const int64_t id = a.id_bits == 32 ? (int64_t)static_cast<const int32_t*>(a.ids)[i]
+                                       : static_cast<const int64_t*>(a.ids)[i];
+    const bool ok = id >= 0 && (uint64_t)id < a.table_rows;
+    if (!ok && id != -1 && blockIdx.x == 0) report(err, TESSA_DEVERR_BAD_ROW);
+    return ok ? (uint32_t)id : none;
+  };
+  if (blockIdx.x >= sum_blocks) {
+    // rows [first, first + rows) of the table, vectors of VE
+    const uint32_t parts = gridDim.x - sum_blocks, part = blockIdx.x - sum_blocks;
+    const uint32_t per = (uint32_t)((a.table_rows + parts - 1u) / parts);
+    const uint64_t first = (uint64_t)part * per;
+    if (first >= a.table_rows) return;
+    const uint32_t rows = (uint32_t)min((uint64_t)per, a.table_rows - first);
+    for (uint32_t i = tid; i < (rows + 31u) / 32u; i += 256u) few_smem[i] = 0u;
+    __syncthreads();
+    for (uint32_t i = tid; i < count; i += 256u) {
+      const uint64_t r = (uint64_t)key_of(i) - first;  // (past the end for padding and other blocks' rows)
+      if (r < rows) atomicOr(few_smem + r / 32u, 1u << (r % 32u));
+    }
+    __syncthreads();
+    const uint32_t vecs = a.dim / VE;
+    Vec<O, VE> zero;
+#pragma unroll
+    for (int i = 0; i < VE; ++i) zero.v[i] = from_f32<O>(0.0f);
+    for (uint64_t i = tid; i < (uint64_t)rows * vecs; i += 256u) {
+      const uint32_t r = (uint32_t)(i / vecs), v = (uint32_t)(i - (uint64_t)r * vecs);
+      if (!(few_smem[r / 32u] >> (r % 32u) & 1u)) *grad_at<O, VE>(a, (uint32_t)first + r, v * VE) = zero;
+    }
+    return;
+  }
+
+  const uint32_t padded = (count + 127u) / 128u * 128u;
+  uint32_t* keys = few_smem;
+  __shared__ uint32_t shared_entry[kFewWarps];  // entries whose key many have
+  __shared__ float part_sum[kFewWarps][32 * VE];
+  for (uint32_t i = tid; i < padded; i += 256u) keys[i] = i < count ? key_of(i) : none;
+  __syncthreads();
+  const uint4* four = reinterpret_cast<const uint4*>(keys);
+  // bits 0..3: which of keys [base + 4 lane, + 4) are k, at or behind `from`
+  auto matches = [&](uint32_t base, uint32_t k, uint32_t from) {
+    const uint4 q = four[base / 4u + lane];
+    const uint32_t m = (q.x == k ? 1u : 0u) | (q.y == k ? 2u : 0u) | (q.z == k ? 4u : 0u) | (q.w == k ? 8u : 0u);
+    const uint32_t j = base + 4u * lane;
+    return j >= from ? m : from - j < 4u ? m & (15u << (from - j)) : 0u;
+  };
+  const T* dout = static_cast<const T*>(a.dout);
+  // adds the rows at lanes' positions 0 .. n - 1, in order, columns col ..
+  auto add_rows = [&](float (&acc)[VE], uint32_t mine, uint32_t n, uint32_t col) {
+    for (uint32_t b = 0; b < n; b += 4u) {
+      Vec<T, VE> x[4];
+#pragma unroll
+      for (uint32_t q = 0; q < 4; ++q) {
+        const uint32_t j = __shfl_sync(0xffffffffu, mine, (b + q) % 32u);
+        if (b + q < n && col < a.dim) x[q] = *reinterpret_cast<const Vec<T, VE>*>(dout + (uint64_t)j * a.dout_stride + col);
+      }
+#pragma unroll
+      for (uint32_t q = 0; q < 4; ++q) {
+        if (b + q >= n || col >= a.dim) break;
+#pragma unroll
+        for (int i = 0; i < VE; ++i) acc[i] += to_f32(x[q].v[i]);
+      }
+    }
+  };
+  const uint32_t t = blockIdx.x * kFewWarps + warp;
+  const uint32_t k = t < count ? keys[t] : none;
+  bool first = k != none;
+  for (uint32_t base = 0; first && base < t; base += 128u) {
+    const uint32_t m = matches(base, k, 0u), j = base + 4u * lane;
+    const uint32_t earlier = j >= t ? 0u : t - j < 4u ? m & ((1u << (t - j)) - 1u) : m;
+    first = !__any_sync(0xffffffffu, earlier != 0u);
+  }
+  uint32_t found = 0, mine = 0;  // lane i: position of the i-th
+  if (first) {
+    for (uint32_t base = t / 128u * 128u; base < count; base += 128u) {
+      const uint32_t m = matches(base, k, t);
+      for (uint32_t lanes = __ballot_sync(0xffffffffu, m != 0u); lanes; lanes &= lanes - 1u) {
+        const uint32_t l = __ffs(lanes) - 1u;
+        for (uint32_t bits = __shfl_sync(0xffffffffu, m, l); bits; bits &= bits - 1u, ++found)
+          if (lane == found) mine = base + 4u * l + __ffs(bits) - 1u;
+      }
+    }
+  }
+  if (lane == 0) shared_entry[warp] = found > 32u ? t : 0xffffffffu;
+  if (found && found <= 32u) {
+    for (uint32_t c0 = 0; c0 < a.dim; c0 += 32u * VE) {
+      const uint32_t col = c0 + lane * VE;
+      Vec<O, VE> old;
+      if (ACC && col < a.dim) old = *grad_at<O, VE>(a, k, col);
+      float acc[VE];
+#pragma unroll
+      for (int i = 0; i < VE; ++i) acc[i] = 0.0f;
+      add_rows(acc, mine, found, col);
+      if (col < a.dim) store_row<ACC, O, VE>(a, k, col, acc, old);
+    }
+  }
+  __syncthreads();
+  for (uint32_t e = 0; e < kFewWarps; ++e) {
+    const uint32_t from = shared_entry[e];
+    if (from == 0xffffffffu) continue;
+    const uint32_t key = keys[from];
+    // this warp's part of the entries, a multiple of 128
+    const uint32_t per = (padded / 128u + kFewWarps - 1u) / kFewWarps * 128u;
+    const uint32_t lo = warp * per, hi = min(padded, lo + per);
+    for (uint32_t c0 = 0; c0 < a.dim; c0 += 32u * VE) {
+      const uint32_t col = c0 + lane * VE;
+      float acc[VE];
+#pragma unroll
+      for (int i = 0; i < VE; ++i) acc[i] = 0.0f;
+      uint32_t n = 0, at = 0;
+      for (uint32_t base = lo; base < hi; base += 128u) {
+        const uint32_t m = matches(base, key, from);
+        for (uint32_t lanes = __ballot_sync(0xffffffffu, m != 0u); lanes; lanes &= lanes - 1u) {
+          const uint32_t l = __ffs(lanes) - 1u;
+          for (uint32_t bits = __shfl_sync(0xffffffffu, m, l); bits; bits &= bits - 1u) {
+            if (lane == n) at = base + 4u * l + __ffs(bits) - 1u;
+            if (++n == 32u) {
+              add_rows(acc, at, 32u, col);
+              n = 0;
+            }
+          }
+        }
+      }
+      add_rows(acc, at, n, col);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) part_sum[warp][lane * VE + i] = acc[i];
+      __syncthreads();
+      if (warp == 0 && col < a.dim) {
+        Vec<O, VE> old;
+        if (ACC) old = *grad_at<O, VE>(a, key, col);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          acc[i] = part_sum[0][lane * VE + i];
+          for (uint32_t w = 1; w < kFewWarps; ++w) acc[i] += part_sum[w][lane * VE + i];
+        }
+        store_row<ACC, O, VE>(a, key, col, acc, old);
+      }
+      __syncthreads();
+    }
+  }
+}
+
 template <class F>
 cudaError_t with_width(uint32_t ve, F f) {
   switch (ve) {
@@ -587,7 +722,7 @@ cudaError_t launch_embedding_lookup(const tessa_lookup_args& a, const AsyncCtx& 
 }
 
 uint64_t embedding_grad_workspace(uint64_t count, uint64_t table_rows, uint32_t dim) {
-  return count ? train::grad_space(count, table_rows, dim).bytes : 0;
+  return count && !train::unsorted(count, dim) ? train::grad_space(count, table_rows, dim).bytes : 0;
 }
 
 cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspace, const AsyncCtx& c,
@@ -600,15 +735,40 @@ cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspa
   // f32 39 instead of 43; 120000 x 256 f32, 117 MB, 46 either way).  A larger
   // gradient is cleared first, at the memory's rate.
   const uint64_t row_bytes = (uint64_t)a.dim * ob, bytes = a.table_rows * row_bytes;
+  const uint32_t widest = 16u / (eb > ob ? eb : ob);
+  uint32_t ve = vector_elems(a.dout, a.count, a.dim, a.dout_stride, eb, widest);
+  ve = vector_elems(a.grad, a.table_rows, a.dim, a.grad_stride, ob, ve);
+  const bool few = a.count > 0 && unsorted(a.count, a.dim);
   const bool whole = a.table_rows == 1 || a.grad_stride == a.dim;
-  const bool beside = !a.accumulate && a.count > 0 && whole && bytes <= kBeside && bytes % 16 == 0 &&
+  const bool beside = !few && !a.accumulate && a.count > 0 && whole && bytes <= kBeside && bytes % 16 == 0 &&
                       reinterpret_cast<uintptr_t>(a.grad) % 16 == 0;
-  if (!a.accumulate && !beside) {
+  const bool clears = few && !a.accumulate && bytes <= kBeside;
+  if (!a.accumulate && !beside && !clears) {
     const cudaError_t e = whole ? cudaMemsetAsync(a.grad, 0, bytes, stream)
                                 : cudaMemset2DAsync(a.grad, a.grad_stride * ob, 0, row_bytes, a.table_rows, stream);
     if (e != cudaSuccess) return e;
   }
   if (a.count == 0) return cudaSuccess;
+  if (few) {
+    const uint32_t sums = (uint32_t)div_up(a.count, kFewWarps);
+    // a block clears 32 KB at least; its bitmap is of a part of the rows
+    const uint64_t want = div_up(bytes, 32768), most = (uint64_t)c.sm_count * 4;
+    const uint32_t clear = clears ? (uint32_t)(want < most ? want : most) : 0u;
+    const uint64_t keys = div_up(a.count, 128) * 512, map = clear ? div_up(div_up(a.table_rows, clear), 32) * 4 : 0;
+    const uint32_t smem = (uint32_t)(keys > map ? keys : map);
+    return with_type(a.dtype, [&](auto t) {
+      return with_type(a.grad_dtype, [&](auto o) {
+        return with_width(ve, [&](auto w) {
+          constexpr int VE = decltype(w)::value;
+          if (a.accumulate)
+            few_ids_kernel<decltype(t), decltype(o), VE, true><<<sums, 256, smem, stream>>>(a, sums, c.err);
+          else
+            few_ids_kernel<decltype(t), decltype(o), VE, false><<<sums + clear, 256, smem, stream>>>(a, sums, c.err);
+          return cudaGetLastError();
+        });
+      });
+    });
+  }
   const GradSpace g = grad_space(a.count, a.table_rows, a.dim);
   const SortPlan p = sort_plan(a.count, a.table_rows);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -633,13 +793,7 @@ cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspa
     return (uint32_t)(want < (uint64_t)c.sm_count ? want : (uint64_t)c.sm_count);
   };
   uint32_t out = 0;
-  if (a.count <= kSmallSort) {
-    s.out_keys = at(g.keys[0]);
-    s.out_pos = at(g.pos[0]);
-    s.blocks = 1;
-    const uint32_t extra = share(0, 1) * 4u;
-    sort_small_kernel<<<1 + extra, kSmallThreads, 0, stream>>>(s);
-  } else if (a.count <= kClusterMost) {
+  if (a.count <= kClusterMost) {
     const uint32_t ctas = (uint32_t)div_up(a.count, kClusterChunk);
     s.out_keys = at(g.keys[0]);
     s.out_pos = at(g.pos[0]);
@@ -705,9 +859,6 @@ cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspa
   m.tile = a.count <= kFewIds ? kShortTile : kTile;
   m.tiles = (uint32_t)div_up(a.count, m.tile);
   m.table_rows = (uint32_t)a.table_rows;
-  const uint32_t most = 16u / (eb > ob ? eb : ob);
-  uint32_t ve = vector_elems(a.dout, a.count, a.dim, a.dout_stride, eb, most);
-  ve = vector_elems(a.grad, a.table_rows, a.dim, a.grad_stride, ob, ve);
   while (ve > 1 && 32u * ve > a.dim) ve >>= 1;  // narrow rows: every lane a column rather than wide accesses
   m.chunks = (uint32_t)div_up(a.dim, 32u * ve);
   const uint32_t grid = (uint32_t)div_up((uint64_t)m.tiles * m.chunks, 8);

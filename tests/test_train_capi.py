@@ -37,7 +37,7 @@ def test_workspace_sizes():
         return n.value
 
     assert grad(0, 10, 10) == 0
-    assert 0 < grad(1, 10, 10) <= grad(1000, 10, 10) < grad(1000, 10, 1000) < grad(100_000, 10, 1000)
+    assert grad(1, 10, 10) <= grad(1000, 10, 10) <= grad(10_000, 10, 10) < grad(10_000, 10, 1000) < grad(100_000, 10, 1000)
     assert grad(100_000, 1000, 64) % 256 == 0
 
     def distill(rows, vocab, k, grad_at):
@@ -73,11 +73,13 @@ def test_refusals_before_any_launch():
         refused(lib.tessa_embedding_lookup, C.LookupArgs(*good[:at], v, *good[at + 1:]), None, code=UNSUPPORTED)
 
     # dout, stride, dim, type, ids, bits, grad type, count, scale, accumulate, grad, stride, rows
-    good = [p, 64, 64, 0, q, 32, 0, 16, 1.0, 0, p + 65536, 64, 64]
+    good = [p, 8, 8, 0, q, 32, 0, 4096 + 904, 1.0, 0, p + 196608, 8, 64]
+    i5 = torch.zeros(5000, dtype=torch.int32, device="cuda")
+    good[4] = i5.data_ptr()
     need = ctypes.c_uint64()
-    C.check(lib.tessa_embedding_grad_workspace(16, 64, 64, need))
+    C.check(lib.tessa_embedding_grad_workspace(5000, 64, 8, need))
     assert lib.tessa_embedding_grad(h, C.LookupGradArgs(*good), w, need.value, None) == 0
-    for at, v in ((0, None), (1, 63), (3, 3), (5, 8), (9, 2), (10, None), (11, 63)):
+    for at, v in ((0, None), (1, 7), (3, 3), (5, 8), (9, 2), (10, None), (11, 7)):
         refused(lib.tessa_embedding_grad, C.LookupGradArgs(*good[:at], v, *good[at + 1:]), w, need.value, None)
     for space, size in ((None, need.value), (w, need.value - 1), (w + 16, need.value)):
         refused(lib.tessa_embedding_grad, C.LookupGradArgs(*good), space, size, None)
