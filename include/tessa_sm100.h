@@ -718,9 +718,9 @@ TESSA_API int tessa_embedding_lookup(tessa_ctx* ctx, const tessa_lookup_args* ar
 /* Gradient of tessa_embedding_lookup: grad[v] = scale * sum of dout[t] over
  * the t with ids[t] == v, for every row v of the table (rows that no id names
  * become zero), or, with accumulate, grad[v] += that sum (rows that no id
- * names are not touched).  The ids are sorted by (id, t), and each row's sum
- * runs over its t in that order in f32 with one rounding at the end: the same
- * inputs give the same bits. */
+ * names are not touched).  A row's terms are added in f32 in an order that the
+ * ids alone decide, with one rounding at the end: the same inputs give the same
+ * bits. */
 typedef struct tessa_lookup_grad_args {
   const void* dout;             /* count x dim */
   uint64_t dout_stride;

@@ -5,16 +5,16 @@
 //
 // Gradient: grad[v] = s * sum_{t: id_t = v} dout[t].  Atomic adds would give
 // another order, and other bits, every time, and a popular row would serialise
-// them.  A few thousand entries are compared with one another (below); more
-// (id, t) are sorted (stable radix sort, digits of at
-// most 10 bits), cut into tiles of 32 sorted entries, and one warp sums a
-// tile's rows run by run in f32: a run inside the tile is written at once, a
-// run that crosses a tile border leaves its part in the workspace, and a last
-// kernel adds each such run's parts.  Every tile holds 32 entries however
-// popular one id is, so skew costs nothing but the parts.  131072 rows of 128
-// f32 into 200000: 67 us, of which the sort 24 (latency; the rows that no id
-// names are cleared beside it), the tiles 17 (4 TB/s), parts 9; adding to the
-// gradient instead 51.
+// them.  Some thousand entries are compared with one another, in one launch.
+// More are sorted as (id, t) (stable radix sort, digits of at most 10 bits) and
+// cut into tiles of 32 sorted entries (8 of fewer entries), and one warp sums a
+// tile's rows run by run in f32: a run inside the tile is written at once, a run
+// that crosses a tile border leaves its part in the workspace, and a last kernel
+// adds each such run's parts.  Every tile holds as many entries however popular
+// one id is, so skew costs nothing but the parts.  131072 rows of 128 f32 into
+// 200000: 67 us, of which the sort 24 (latency; the rows that no id names are
+// cleared beside it), the tiles 17 (4 TB/s), parts 9; adding to the gradient
+// instead 51.
 #include "train_common.cuh"
 
 namespace tessa {
@@ -512,8 +512,8 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(const tessa_lookup_grad_
 // each a part of the entries, whose sums are added in order.  Blocks behind
 // these clear the rows that no id names, which they mark in a bitmap, so one
 // launch does it all: 256 ids over 20000 x 128 f32 4.2 us, by sorting 11.5; over
-// 200000 19 and 23, mostly clearing.  Bound by
-// the latency of three dependent reads, and by an id's rows where it has many.
+// 200000 19 and 23, mostly clearing.  Bound by the latency of three dependent
+// reads, and by an id's rows where it has many.
 constexpr uint32_t kFewWarps = 8;
 
 template <class T, class O, int VE, bool ACC>

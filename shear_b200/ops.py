@@ -909,7 +909,8 @@ def embedding_grad(dout, ids, table_rows: int, scale: float = 1.0, out_dtype=Non
                    accumulate: bool = False, ctx: Context | None = None):
     """Gradient of :func:`embedding_lookup` with respect to the table
     (tessa_embedding_grad): ``grad[v] = scale * sum(dout[t] for ids[t] == v)``,
-    each row summed in f32 in the order of t, so equal inputs give equal bits.
+    each row summed in f32 in an order that the ids alone decide, so equal
+    inputs give equal bits.
 
     dout [..., dim] (ids.shape + (dim,), or [ids.numel(), dim] with any row
     stride).  Returns [table_rows, dim] in out_dtype (default dout's).  With
