@@ -48,6 +48,31 @@ __global__ void __launch_bounds__(256) lookup_kernel(const tessa_lookup_args a, 
 
 // ------------------------------------------------------------------- sort
 
+// After the one-launch sort the sums are launched ahead of its end (programmatic
+// dependent launch): a kernel lets the next one start at once, and waits for all
+// of the one before to be done before it touches memory.  10000 ids over 20000 x
+// 64: 22.5 us a call instead of 25; after the longer sort, 262144 ids, 126 instead
+// of 120.
+__device__ __forceinline__ void after_the_last() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+template <class... Args, class... Given>
+cudaError_t launch_after(bool ahead, void (*kernel)(Args...), uint32_t grid, uint32_t threads, cudaStream_t stream,
+                         Given... given) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = ahead ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, Args(given)...);
+}
+
 constexpr uint32_t kSortThreads = 512;
 constexpr uint32_t kSortWarps = kSortThreads / 32;
 constexpr uint32_t kMaxDigitBits = 10;
@@ -264,6 +289,7 @@ __global__ void __launch_bounds__(kClusterChunk)
   const uint32_t tid = threadIdx.x, warp = tid / 32u, lane = tid % 32u, rank = cluster_ctarank();
   const uint32_t at = rank * kClusterChunk + tid;
   uint16_t* mine = warp_digits + warp * bins;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (rank == 0 && tid < 2u) a.runs[tid] = 0u;
   cluster_sync();  // every CTA has started
   for (uint32_t pass = 0; pass < passes; ++pass) {
@@ -360,6 +386,7 @@ template <class T, class O, int VE, bool ACC, uint32_t TILE>
 __global__ void __launch_bounds__(256) sum_tiles_kernel(const tessa_lookup_grad_args a, const SumArgs s) {
   const uint64_t w = (uint64_t)blockIdx.x * 8u + threadIdx.x / 32u;
   const uint32_t tile = (uint32_t)(w / s.chunks), lane = threadIdx.x % 32u;
+  after_the_last();
   if (tile >= s.tiles) return;
   const uint32_t col = (uint32_t)(w % s.chunks) * 32u * VE + lane * VE;
   const bool in = col < a.dim;
@@ -435,6 +462,7 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(const tessa_lookup_grad_
   const uint32_t pieces = (s.part_stride + 127u) / 128u;
   const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
   __shared__ float4 sums[256];
+  after_the_last();
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   auto add = [&](const float4& v) {
     acc.x += v.x;
@@ -866,23 +894,21 @@ cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspa
     return with_type(a.grad_dtype, [&](auto o) {
       return with_width(ve, [&](auto w) {
         constexpr int VE = decltype(w)::value;
+        const bool ahead = a.count <= kClusterMost;
         auto tiles = [&](auto tile, auto add) {
-          sum_tiles_kernel<decltype(t), decltype(o), VE, decltype(add)::value, decltype(tile)::value>
-              <<<grid, 256, 0, stream>>>(a, m);
+          return launch_after(ahead, sum_tiles_kernel<decltype(t), decltype(o), VE, decltype(add)::value, decltype(tile)::value>,
+                              grid, 256, stream, a, m);
         };
-        auto either = [&](auto tile) {
-          if (a.accumulate) tiles(tile, std::true_type());
-          else tiles(tile, std::false_type());
-        };
-        if (m.tile == kTile) either(std::integral_constant<uint32_t, kTile>());
-        else either(std::integral_constant<uint32_t, kShortTile>());
-        if (m.tiles > 1) {
+        auto either = [&](auto tile) { return a.accumulate ? tiles(tile, std::true_type()) : tiles(tile, std::false_type()); };
+        cudaError_t e = m.tile == kTile ? either(std::integral_constant<uint32_t, kTile>())
+                                        : either(std::integral_constant<uint32_t, kShortTile>());
+        if (e == cudaSuccess && m.tiles > 1) {
           const uint64_t items = div_up((uint64_t)m.tiles * div_up(a.dim, 128), 8), most = (uint64_t)c.sm_count * 8;
           const uint32_t blocks = (uint32_t)(items < most ? items : most);
-          if (a.accumulate) sum_parts_kernel<decltype(o), true><<<blocks, 256, 0, stream>>>(a, m);
-          else sum_parts_kernel<decltype(o), false><<<blocks, 256, 0, stream>>>(a, m);
+          e = a.accumulate ? launch_after(ahead, sum_parts_kernel<decltype(o), true>, blocks, 256, stream, a, m)
+                           : launch_after(ahead, sum_parts_kernel<decltype(o), false>, blocks, 256, stream, a, m);
         }
-        return cudaGetLastError();
+        return e;
       });
     });
   });
