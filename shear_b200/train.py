@@ -145,18 +145,24 @@ class TableTrainer:
             raise ValueError("temperature must be positive")
         self.table, self.rate, self.temperature, self.scale = table, rate, temperature, scale
 
+    def _named(self, ids):
+        """Which ids name a row of the table."""
+        return (ids >= 0) & (ids < self.table.shape[0])
+
     def scores(self, ids):
         """scale * table[ids] . table^T in bf16, each row's own score -inf; and the codes that its gradient needs."""
         x = ops.embedding_lookup(self.table, ids, self.scale)
         xq, wq = ops.quantize_fp8_both(x), ops.quantize_fp8_both(self.table)
         z = ops.matmul_fp8(*xq[:2], *wq[:2], out_dtype=torch.bfloat16)
-        z.scatter_(1, ids.clamp(min=0).long().unsqueeze(1), float("-inf"))
+        if z.shape[1]:  # (the row of an id outside the table takes no part, whichever of its scores this hides)
+            z.scatter_(1, ids.long().clamp(0, z.shape[1] - 1).unsqueeze(1), float("-inf"))
         return z, xq[2:], wq[2:]
 
     def step(self, ids, teacher_ids, teacher_logits):
-        """One step on the batch; returns its mean loss (a device scalar).  Rows of id -1 take no part."""
+        """One step on the batch; returns its mean loss (a device scalar).  Rows of id -1 take
+        no part, nor do those of an id outside the table, which the next call reports."""
         z, x_t, w_t = self.scores(ids)
-        weights = (ids >= 0).float()
+        weights = self._named(ids).float()
         weights /= weights.sum().clamp(min=1.0)
         loss, _, dz = ops.distill_topk_grad(z, teacher_ids, teacher_logits, self.temperature, weights, out=z)
         c, s, ct, st = ops.quantize_fp8_both(dz)

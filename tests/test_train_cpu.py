@@ -1,0 +1,91 @@
+"""The trainer and the differentiable functions with plain torch in place of
+the kernels, so that they run without a GPU."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+def _rows_of(ids, rows):
+    return (ids >= 0) & (ids < rows)
+
+
+def _lookup(table, ids, scale=1.0, **_):
+    ok = _rows_of(ids, table.shape[0])
+    if not table.shape[0]:
+        return table.new_zeros(*ids.shape, table.shape[1])
+    return torch.where(ok.unsqueeze(-1), scale * table[torch.where(ok, ids, 0).long()], 0.0)
+
+
+def _lookup_grad(dout, ids, table_rows, scale=1.0, out=None, accumulate=False, **_):
+    ok = _rows_of(ids, table_rows)
+    if out is None:
+        out = dout.new_zeros(table_rows, dout.shape[-1])
+    return out.index_add_(0, ids[ok].long(), scale * dout[ok])
+
+
+def _codes(x, transpose=False, **_):
+    return (x.t(), None) if transpose else (x, None)
+
+
+def _product(a, a_scales, b, b_scales, out_dtype=None, **_):
+    return a.float() @ b.float().t()
+
+
+def _distill(logits, teacher_ids, teacher_logits, temperature=1.0, row_weights=None, out=None, **_):
+    rows, vocab = logits.shape
+    w = torch.ones(rows) if row_weights is None else row_weights
+    loss, lse, grad = torch.zeros(rows), torch.full((rows,), float("-inf")), torch.zeros(rows, vocab)
+    for r in range(rows):
+        there = _rows_of(teacher_ids[r], vocab) & (teacher_logits[r] > float("-inf"))
+        if not there.any():
+            continue
+        ids, x = teacher_ids[r][there].long(), logits[r].float() / temperature
+        log_p, log_q = torch.log_softmax(teacher_logits[r][there] / temperature, 0), torch.log_softmax(x, 0)
+        loss[r] = temperature ** 2 * (log_p.exp() * (log_p - log_q[ids])).sum()
+        lse[r] = torch.logsumexp(x, 0)
+        grad[r] = w[r] * temperature * log_q.exp().index_add(0, ids, -log_p.exp())
+    if out is not None:
+        grad = out.copy_(grad)
+    return loss, lse, grad
+
+
+@pytest.fixture
+def train(monkeypatch):
+    from shear_b200 import train
+    plain = {"embedding_lookup": _lookup, "embedding_grad": _lookup_grad, "quantize_fp8": _codes,
+             "quantize_fp8_both": lambda x, **k: (*_codes(x), *_codes(x, True)), "matmul_fp8": _product,
+             "distill_topk_grad": _distill, "distill_topk": lambda *a, **k: _distill(*a, **k)[:2]}
+    for name, f in plain.items():
+        monkeypatch.setattr(train.ops, name, f)
+    return train
+
+
+def _trainer(train, rows=12, dim=5):
+    g = torch.Generator().manual_seed(0)
+    ids = torch.stack([torch.randperm(rows, generator=g)[:4] for _ in range(6)]).int()
+    return (train.TableTrainer(torch.randn(rows, dim, generator=g), 0.1, 1.5, 0.5), ids,
+            torch.randn(6, 4, generator=g))
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("bad", [12, 2 ** 31 - 1, -7])
+def test_an_id_outside_the_table_takes_no_part(train, bad, dtype):
+    batch = torch.tensor([3, bad, 0, 5, bad, 11], dtype=dtype)
+    runs = []
+    for b in (batch, torch.where(batch == bad, -1, batch)):
+        trainer, ids, logits = _trainer(train)
+        # no list names its own row, nor the first or last one
+        ids = torch.where((ids == batch.unsqueeze(1)) | (ids == 0) | (ids == 11), -1, ids)
+        runs.append((trainer.step(b, ids, logits), trainer.table, trainer.scores(b)[0]))
+    for x, y in zip(runs[0][:2], runs[1][:2]):
+        assert torch.equal(x, y) and x.isfinite().all()
+    ok = (batch != bad).nonzero()[:, 0]
+    z = runs[0][2]
+    assert torch.equal(z[ok], runs[1][2][ok])
+    assert torch.equal((z == float("-inf")).nonzero()[:, 1][ok], batch[ok].long())  # a row's own score alone
+
+
+def test_a_table_without_rows(train):
+    trainer = train.TableTrainer(torch.zeros(0, 5), 0.1)
+    batch = torch.full((3,), -1, dtype=torch.int32)
+    assert float(trainer.step(batch, batch.unsqueeze(1), torch.zeros(3, 1))) == 0.0

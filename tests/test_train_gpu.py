@@ -196,3 +196,29 @@ def test_the_command_learns():
     assert run.returncode == 0, run.stderr[-2000:]
     r = json.loads(run.stdout.strip().splitlines()[-1])
     assert r["loss_last"] < 0.7 * r["loss_first"] and r["recall_after"] > r["recall_before"] + 0.1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [500, 2 ** 31 - 1, -2])
+def test_an_id_outside_the_table_is_reported(bad):
+    # the step, or the wait behind it, raises; the device goes on, and so does the table
+    import torch
+    from shear_b200 import ops
+    from shear_b200._capi import TessaError
+    trainer, ids, logits = _trainer()
+    start = trainer.table.clone()
+    batch = torch.arange(40, device="cuda").int()
+    want = trainer.step(batch, ids[:40], logits[:40]), trainer.table.clone()
+    trainer.table.copy_(start)
+    wrong = batch.clone()
+    wrong[7] = bad
+    with pytest.raises(TessaError) as e:
+        trainer.step(wrong, ids[:40], logits[:40])
+        ops.async_status()
+    assert e.value.code == -5
+    torch.cuda.synchronize()
+    assert trainer.table.isfinite().all()
+    trainer.table.copy_(start)
+    got = trainer.step(batch, ids[:40], logits[:40])
+    ops.async_status()
+    assert torch.equal(got, want[0]) and torch.equal(trainer.table, want[1])
