@@ -162,7 +162,11 @@ class TableTrainer:
         """One step on the batch; returns its mean loss (a device scalar).  Rows of id -1 take
         no part, nor do those of an id outside the table, which the next call reports."""
         z, x_t, w_t = self.scores(ids)
-        weights = self._named(ids).float()
+        named = self._named(ids)
+        # a padding row's list may hold anything, an entry of the hidden score among
+        # it, of which the loss is infinite: only without entries it takes no part
+        teacher_ids = teacher_ids.masked_fill(~named.unsqueeze(1), -1)
+        weights = named.float()
         weights /= weights.sum().clamp(min=1.0)
         loss, _, dz = ops.distill_topk_grad(z, teacher_ids, teacher_logits, self.temperature, weights, out=z)
         c, s, ct, st = ops.quantize_fp8_both(dz)
@@ -175,6 +179,7 @@ class TableTrainer:
     def recall(self, ids, teacher_ids) -> float:
         """Share of the teacher's neighbours of these rows among the table's own first k."""
         z = self.scores(ids)[0]
+        teacher_ids = teacher_ids.masked_fill(~self._named(ids).unsqueeze(1), -1)
         got = z.topk(teacher_ids.shape[1], dim=1).indices.int()
         hit = (got.unsqueeze(2) == teacher_ids.unsqueeze(1)).any(1) & (teacher_ids >= 0)
         return float(hit.sum() / (teacher_ids >= 0).sum().clamp(min=1))

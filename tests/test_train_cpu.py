@@ -89,3 +89,21 @@ def test_a_table_without_rows(train):
     trainer = train.TableTrainer(torch.zeros(0, 5), 0.1)
     batch = torch.full((3,), -1, dtype=torch.int32)
     assert float(trainer.step(batch, batch.unsqueeze(1), torch.zeros(3, 1))) == 0.0
+
+
+@pytest.mark.parametrize("filler", [0.0, float("nan"), float("inf")])
+def test_padding_rows_take_no_part_whatever_their_lists(train, filler):
+    # the lists of padding rows name every row, and hold anything
+    trainer, ids, logits = _trainer(train)
+    start, batch = trainer.table.clone(), torch.tensor([3, 8, 5], dtype=torch.int32)
+    lists = torch.where(ids[:3] == batch.unsqueeze(1), -1, ids[:3])
+    want = trainer.step(batch, lists, logits[:3]), trainer.table.clone()
+    share = trainer.recall(batch, lists)
+    trainer.table.copy_(start)
+    padded = torch.tensor([-1, 3, -1, 8, 5, -1], dtype=torch.int32)
+    all_lists, all_logits = torch.arange(12).int().view(3, 4).repeat(2, 1), torch.full((6, 4), filler)
+    all_lists[padded >= 0], all_logits[padded >= 0] = lists, logits[:3]
+    got = trainer.step(padded, all_lists, all_logits), trainer.table
+    for x, y in zip(got, want):
+        assert x.isfinite().all() and torch.allclose(x, y, rtol=1e-5, atol=1e-6)
+    assert trainer.recall(padded, all_lists) == share

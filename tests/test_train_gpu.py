@@ -222,3 +222,20 @@ def test_an_id_outside_the_table_is_reported(bad):
     got = trainer.step(batch, ids[:40], logits[:40])
     ops.async_status()
     assert torch.equal(got, want[0]) and torch.equal(trainer.table, want[1])
+
+
+@pytest.mark.gpu
+def test_padding_rows_with_lists_of_anything():
+    import torch
+    trainer, ids, logits = _trainer()
+    start = trainer.table.clone()
+    batch = torch.arange(100, 140, device="cuda").int()
+    want = trainer.step(batch, ids[100:140], logits[100:140]), trainer.table.clone()
+    padded = torch.cat([batch, torch.full((24,), -1, device="cuda", dtype=torch.int32)])
+    lists = torch.cat([ids[100:140], torch.arange(8, device="cuda").int().repeat(24, 1)])  # id 0 among them
+    for filler in (0.0, float("nan"), float("inf")):
+        trainer.table.copy_(start)
+        loss = trainer.step(padded, lists, torch.cat([logits[100:140], torch.full((24, 8), filler, device="cuda")]))
+        # the same sums, of which the products' may be split otherwise (bf16 scores, FP8 codes of a step's size)
+        assert torch.allclose(loss, want[0], rtol=1e-4)
+        assert torch.allclose(trainer.table, want[1], rtol=0, atol=float((want[1] - start).abs().max()) / 16)
