@@ -703,7 +703,7 @@ typedef struct tessa_lookup_args {
   const void* table;
   uint64_t table_rows;          /* below 2^32 - 1 */
   uint64_t table_stride;
-  uint32_t dim;
+  uint32_t dim;                 /* at most 2^32 - 1024 */
   uint32_t dtype;
   const void* ids;
   uint32_t id_bits;             /* 32 or 64 */
@@ -724,7 +724,7 @@ TESSA_API int tessa_embedding_lookup(tessa_ctx* ctx, const tessa_lookup_args* ar
 typedef struct tessa_lookup_grad_args {
   const void* dout;             /* count x dim */
   uint64_t dout_stride;
-  uint32_t dim;
+  uint32_t dim;                 /* at most 2^32 - 1024 */
   uint32_t dtype;
   const void* ids;
   uint32_t id_bits;

@@ -71,6 +71,12 @@ int launched(const char* what, cudaError_t e) {
 constexpr uint64_t kMaxIds = 1ull << 31;          // sorted positions are 32-bit
 constexpr uint64_t kMaxMatrix = (1ull << 31) - 1;  // TMA coordinates and tile counts are 32-bit
 constexpr uint64_t kMaxTableRows = 0xfffffffeull;  // one key above the last row marks padding
+constexpr uint32_t kMaxDim = 0xfffffc00u;          // columns are counted in 32 bits, by steps of up to 256
+
+int check_dim(uint32_t dim) {
+  if (dim > kMaxDim) return bad(TESSA_ERR_UNSUPPORTED, "rows of %u columns: at most 2^32 - 1024", dim);
+  return TESSA_OK;
+}
 
 }  // namespace
 
@@ -82,6 +88,7 @@ int tessa_embedding_lookup(tessa_ctx* ctx, const tessa_lookup_args* args, void* 
   TRY(check_matrix("table", a.table, a.table_rows, a.dim, a.table_stride, a.dtype));
   TRY(check_matrix("out", a.out, a.count, a.dim, a.out_stride, a.out_dtype));
   TRY(check_ids(a.ids, a.id_bits, a.count));
+  TRY(check_dim(a.dim));
   if (a.table_rows > kMaxTableRows) return bad(TESSA_ERR_UNSUPPORTED, "table of %llu rows", (ull)a.table_rows);
   if (a.count >= kMaxIds) return bad(TESSA_ERR_UNSUPPORTED, "%llu ids: below 2^31 are supported", (ull)a.count);
   AsyncCtx c;
@@ -92,6 +99,7 @@ int tessa_embedding_lookup(tessa_ctx* ctx, const tessa_lookup_args* args, void* 
 
 int tessa_embedding_grad_workspace(uint64_t count, uint64_t table_rows, uint32_t dim, uint64_t* bytes) {
   if (!bytes) return bad(TESSA_ERR_INVALID_ARG, "null argument");
+  TRY(check_dim(dim));
   *bytes = embedding_grad_workspace(count, table_rows, dim);
   return TESSA_OK;
 }
@@ -103,6 +111,7 @@ int tessa_embedding_grad(tessa_ctx* ctx, const tessa_lookup_grad_args* args, voi
   TRY(check_matrix("dout", a.dout, a.count, a.dim, a.dout_stride, a.dtype));
   TRY(check_matrix("grad", a.grad, a.table_rows, a.dim, a.grad_stride, a.grad_dtype));
   TRY(check_ids(a.ids, a.id_bits, a.count));
+  TRY(check_dim(a.dim));
   if (a.accumulate > 1) return bad(TESSA_ERR_INVALID_ARG, "accumulate %u: 0 or 1", a.accumulate);
   if (a.table_rows > kMaxTableRows) return bad(TESSA_ERR_UNSUPPORTED, "table of %llu rows", (ull)a.table_rows);
   if (a.count >= kMaxIds) return bad(TESSA_ERR_UNSUPPORTED, "%llu ids: below 2^31 are supported", (ull)a.count);

@@ -106,3 +106,27 @@ def test_refusals_before_any_launch():
         got = lib.tessa_distill_topk(h, C.DistillArgs(*good[:at], v, *good[at + 1:]), None, 0, None)
         assert got in (INVALID, UNSUPPORTED), (at, v, got)
     ops.async_status()
+
+
+def test_workspace_of_rows_too_long_to_count():
+    # columns are counted in 32 bits: rows whose last step would wrap around are refused
+    lib = C.load()
+    n = ctypes.c_uint64()
+    assert lib.tessa_embedding_grad_workspace(10_000, 2, 0xfffffc00, n) == 0
+    assert n.value >= 10_000 // 32 * 2 * 0xfffffc00 * 4
+    for dim in (0xfffffc01, 0xfffffffd, 0xffffffff):
+        assert lib.tessa_embedding_grad_workspace(10_000, 2, dim, n) == UNSUPPORTED
+
+
+@pytest.mark.gpu
+def test_rows_too_long_to_count():
+    # refused before any launch, so that no memory of that size has to be there
+    import torch
+    from shear_b200 import ops
+    lib, h = C.load(), ops.context(0).handle
+    t = torch.zeros(4096, device="cuda")
+    p = t.data_ptr()
+    for dim in (0xfffffc01, 0xffffffff):
+        assert lib.tessa_embedding_lookup(h, C.LookupArgs(p, 1, dim, dim, 0, p, 32, 0, 1, 1.0, p, dim), None) == UNSUPPORTED
+        assert lib.tessa_embedding_grad(h, C.LookupGradArgs(p, dim, dim, 0, p, 32, 0, 1, 1.0, 0, p, dim, 1), None, 0,
+                                        None) == UNSUPPORTED
