@@ -349,11 +349,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (rank == 1) {
-      // The pair's MMAs read this CTA's memory until they have all completed.
-      uint32_t dummy = 0u;
-      if (lane == 0) mbar_wait(&drained, 0u, &dummy, p.err, p.timeout_ns);
-    } else {
+    if (rank == 0) {
       // The warp stays together, every operand of an MMA is the same in all
       // lanes and no branch depends on a wait's answer, so that the compiler
       // keeps the operands in uniform registers: an issue from one diverged
@@ -565,6 +561,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  // The pair's MMAs read the second CTA's memory until they have all completed,
+  // too.  Its epilogue has seen the last tile by now, so the wait is as short as
+  // any other: from the kernel's start it would be the whole product's time,
+  // which the limit of one wait says nothing about.
+  if (rank == 1 && threadIdx.x < 32u) {
+    uint32_t dummy = 0u;
+    if (lane == 0) mbar_wait(&drained, 0u, &dummy, p.err, p.timeout_ns);
+    __syncwarp();
+  }
   cluster_sync();  // no arrival, copy or MMA of the peer is under way on this CTA's memory
   tc_fence_after();
   if (warp == 1) tmem_dealloc_pair(tmem, 512);
