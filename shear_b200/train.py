@@ -16,7 +16,8 @@ The teacher's list is what :func:`shear_b200.ops.leaf_topk_sq8` returns: ids
 enqueues work, so it can be captured in a CUDA graph.
 
 :func:`lookup`, :func:`product_fp8` and :func:`distill` are the same operators
-as differentiable torch functions, for models of one's own.
+as differentiable torch functions, for models of one's own.  They have first
+derivatives only: a second one through them raises.
 
 ``python -m shear_b200.train`` runs the whole path on synthetic vectors and
 prints the loss and the share of the teacher's neighbours that the table ranks
@@ -34,6 +35,32 @@ from . import ops
 MAX_ROWS = 65535  # rows of one leaf: teacher_lists compares all of them
 
 
+class _FirstOrder(torch.autograd.Function):
+    """A gradient as it is, for which nothing but an error leads back to what it depends on."""
+
+    @staticmethod
+    def forward(ctx, name, grad, *depends):
+        ctx.name = name
+        return grad.detach()
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError(f"{ctx.name} has no second derivative")
+
+
+def _first_order(name, grad, *depends):
+    """`grad` from a kernel, which leaves no graph: where one is being made
+    (create_graph), a second derivative through it has to fail, not to vanish."""
+    if grad is None or not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in depends):
+        return grad
+    return _FirstOrder.apply(name, grad, *(t for t in depends if t is not None))
+
+
+def _link(t):
+    """An empty tensor that depends on t without holding its memory."""
+    return t[:0].clone()
+
+
 class _Lookup(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, ids, scale):
@@ -44,19 +71,20 @@ class _Lookup(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         (ids,) = ctx.saved_tensors
-        dout = dout.reshape(-1, dout.shape[-1])
-        return ops.embedding_grad(_rows(dout), ids.reshape(-1), ctx.rows, ctx.scale), None, None
+        d2 = _rows(dout.reshape(-1, dout.shape[-1]))
+        grad = ops.embedding_grad(d2, ids.reshape(-1), ctx.rows, ctx.scale)
+        return _first_order("lookup", grad, dout), None, None
 
 
 class _ProductFp8(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, out_dtype):
+    def forward(ctx, x, w, out_dtype, links):
         need_x, need_w = ctx.needs_input_grad[:2]
         # dx needs w's codes along columns, dw those of x
         xc, xs, *x_t = ops.quantize_fp8_both(x) if need_w else ops.quantize_fp8(x)
         wc, ws, *w_t = ops.quantize_fp8_both(w) if need_x else ops.quantize_fp8(w)
         ctx.save_for_backward(*x_t, *w_t)
-        ctx.types = x.dtype, w.dtype
+        ctx.types, ctx.links = (x.dtype, w.dtype), links
         return ops.matmul_fp8(xc, xs, wc, ws, out_dtype=out_dtype)
 
     @staticmethod
@@ -65,7 +93,7 @@ class _ProductFp8(torch.autograd.Function):
         saved = list(ctx.saved_tensors)
         x_t = (saved.pop(0), saved.pop(0)) if need_w else None
         dx = dw = None
-        dy = _rows(dy)
+        given, dy = dy, _rows(dy)
         if need_x and need_w:
             c, s, ct, st = ops.quantize_fp8_both(dy)
         elif need_x:
@@ -76,7 +104,8 @@ class _ProductFp8(torch.autograd.Function):
             dx = ops.matmul_fp8(c, s, *saved, out_dtype=ctx.types[0])
         if need_w:
             dw = ops.matmul_fp8(ct, st, *x_t, out_dtype=ctx.types[1])
-        return dx, dw, None
+        x, w = ctx.links
+        return _first_order("product_fp8", dx, given, w), _first_order("product_fp8", dw, given, x), None, None
 
 
 class _Distill(torch.autograd.Function):
@@ -89,7 +118,8 @@ class _Distill(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dloss):
         logits, ids, teacher = ctx.saved_tensors
-        return ops.distill_topk_grad(logits, ids, teacher, ctx.temperature, row_weights=dloss)[2], None, None, None
+        grad = ops.distill_topk_grad(logits, ids, teacher, ctx.temperature, row_weights=dloss)[2]
+        return _first_order("distill", grad, dloss, logits), None, None, None
 
 
 def _rows(t):
@@ -106,7 +136,8 @@ def product_fp8(x, w, out_dtype=torch.float32):
     """Differentiable ``x . w^T`` of FP8 codes of x [m, k] and w [n, k]
     (:func:`shear_b200.ops.matmul_fp8`): the gradients are products of FP8
     codes too, of the incoming gradient with those of w and of x."""
-    return _ProductFp8.apply(x, w, out_dtype)
+    both = torch.is_grad_enabled() and x.requires_grad and w.requires_grad
+    return _ProductFp8.apply(x, w, out_dtype, (_link(x), _link(w)) if both else (None, None))
 
 
 def distill(logits, teacher_ids, teacher_logits, temperature: float = 1.0):

@@ -56,7 +56,7 @@ def train(monkeypatch):
              "quantize_fp8_both": lambda x, **k: (*_codes(x), *_codes(x, True)), "matmul_fp8": _product,
              "distill_topk_grad": _distill, "distill_topk": lambda *a, **k: _distill(*a, **k)[:2]}
     for name, f in plain.items():
-        monkeypatch.setattr(train.ops, name, f)
+        monkeypatch.setattr(train.ops, name, torch.no_grad()(f))  # as kernels do, they leave no graph
     return train
 
 
@@ -107,3 +107,46 @@ def test_padding_rows_take_no_part_whatever_their_lists(train, filler):
     for x, y in zip(got, want):
         assert x.isfinite().all() and torch.allclose(x, y, rtol=1e-5, atol=1e-6)
     assert trainer.recall(padded, all_lists) == share
+
+
+def _first_order_cases(train):
+    """(name, function of the tensors, tensors): scalars by the three functions."""
+    g = torch.Generator().manual_seed(1)
+    rand = lambda *s: torch.randn(*s, generator=g)
+    ids, lists = torch.tensor([2, 0, 2]), torch.tensor([[0, 3], [1, 2], [4, 1]])
+    return [
+        ("lookup", lambda t: train.lookup(t, ids).pow(3).sum(), (rand(4, 5),)),
+        ("product_fp8", lambda x, w: train.product_fp8(x, w).sum(), (rand(3, 4), rand(5, 4))),
+        ("product_fp8", lambda x: train.product_fp8(x, torch.ones(2, 4)).square().sum(), (rand(3, 4),)),
+        ("product_fp8", lambda w: train.product_fp8(torch.ones(2, 4), w).square().sum(), (rand(3, 4),)),
+        ("distill", lambda z: train.distill(z, lists, torch.ones(3, 2), 1.5).sum(), (rand(3, 5),)),
+    ]
+
+
+@pytest.mark.parametrize("case", range(5))
+def test_a_second_derivative_is_refused_not_lost(train, case):
+    name, f, tensors = _first_order_cases(train)[case]
+    tensors = [t.requires_grad_() for t in tensors]
+    once = torch.autograd.grad(f(*tensors), tensors)
+    grads = torch.autograd.grad(f(*tensors), tensors, create_graph=True)
+    for x, y in zip(grads, once):
+        assert torch.equal(x, y)
+    for g, t in zip(grads, reversed(tensors)):  # with two: each gradient depends on the other tensor
+        with pytest.raises(RuntimeError, match=f"{name} .*second"):
+            torch.autograd.grad(g.square().sum() + tensors[0].sum() + tensors[-1].sum(), t, retain_graph=True)
+        with pytest.raises(RuntimeError, match=f"{name} .*second"):
+            (g.square().sum() + t.sum()).backward(retain_graph=True)
+
+
+def test_a_second_derivative_past_these_functions(train):
+    # what does not depend on their gradients, or is linear, goes through
+    t = torch.randn(4, 3).requires_grad_()
+    (g,) = torch.autograd.grad(train.lookup(t, torch.tensor([1, 1])).sum() + t.pow(3).sum(), t, create_graph=True)
+    (h,) = torch.autograd.grad(g.sum(), t)
+    assert torch.equal(h, 6 * t.detach())
+    x, w, v = (torch.randn(2, 3).requires_grad_() for _ in range(3))
+    y = train.product_fp8(x, w).sum() + v.pow(2).sum()
+    (gv,) = torch.autograd.grad(y, v, create_graph=True)
+    y.backward(create_graph=True)
+    gv.sum().backward()
+    assert torch.equal(v.grad.detach(), 2 * v.detach() + 2)

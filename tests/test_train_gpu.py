@@ -239,3 +239,20 @@ def test_padding_rows_with_lists_of_anything():
         # the same sums, of which the products' may be split otherwise (bf16 scores, FP8 codes of a step's size)
         assert torch.allclose(loss, want[0], rtol=1e-4)
         assert torch.allclose(trainer.table, want[1], rtol=0, atol=float((want[1] - start).abs().max()) / 16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["lookup", "product_fp8", "distill"])
+def test_second_derivatives_are_refused(name):
+    import torch
+    from shear_b200 import train
+    t = torch.randn(6, 32, device="cuda").requires_grad_()
+    w = torch.randn(9, 32, device="cuda").requires_grad_()
+    ids = torch.tensor([[1, 2], [0, 3], [5, 4], [7, 8], [3, 3], [1, 0]], device="cuda")
+    y = {"lookup": lambda: train.lookup(t, ids).square(), "product_fp8": lambda: train.product_fp8(t, w),
+         "distill": lambda: train.distill(t, ids, torch.ones(6, 2, device="cuda"))}[name]().sum()
+    (plain,) = torch.autograd.grad(y, t, retain_graph=True)
+    (g,) = torch.autograd.grad(y, t, create_graph=True)
+    assert torch.equal(g.detach(), plain)
+    with pytest.raises(RuntimeError, match=f"{name} has no second derivative"):
+        torch.autograd.grad(g.square().sum() + t.sum() + w.sum(), w if name == "product_fp8" else t)
