@@ -18,9 +18,9 @@
  *    allocates (device scratch, pinned staging) and frees it in the matching
  *    destroy call.
  *  - `stream` is a cudaStream_t passed as void* (NULL = legacy default stream).
- *  - A context is bound to one device and is not thread-safe: use one context
- *    per GPU per host thread (the reference serialises its CUDA engine behind a
- *    mutex, CB:34666).
+ *  - A context is bound to one device and is not thread-safe (but for the
+ *    calls that train the vectors): use one context per GPU per host thread (the
+ *    reference serialises its CUDA engine behind a mutex, CB:34666).
  *  - Distances follow the reference bit for bit: SQ8 leaf distances are
  *    rn(rn(n_i+n_j) + rn(-2*rn(rn(s_i*s_j)*dot))) clamped at 0 (CB:8987-9002);
  *    leaf lists use the stable eps/id order of CB:7229-7259.
@@ -681,11 +681,13 @@ TESSA_API void tessa_replay_session_destroy(tessa_replay_session* session);
  * device, no scratch is kept in the context (where one is needed the caller
  * passes `workspace`, 256-byte aligned, of the size that the matching
  * *_workspace function gives; it is free again when the call's work is done),
- * and they may be captured into a CUDA graph (after a first call on the context,
- * which sets its error word up).  What a kernel finds wrong (an
- * id outside the table: TESSA_ERR_BAD_ROW; an expired wait: TESSA_ERR_TIMEOUT)
- * is therefore reported by the next of these calls on the context, or by
- * tessa_async_status, which waits for `stream` first; either report clears it.
+ * and they may be captured into a CUDA graph (the context has to outlive it).
+ * What a kernel finds wrong (an id outside the table: TESSA_ERR_BAD_ROW; an
+ * expired wait: TESSA_ERR_TIMEOUT) is therefore reported by the next of these
+ * calls on the context, which then enqueues nothing, or by tessa_async_status,
+ * which waits for `stream` first; either report clears it.  Unlike all others,
+ * these calls and tessa_async_status may be made on one context by several host
+ * threads at once; each error is then reported to one of them.
  * A bad id is never read through: its row counts as padding.
  *
  * Matrices are row-major device memory with `stride` elements from row to row

@@ -284,7 +284,7 @@ struct tessa_ctx {
   DevBuf probe;                     // bounded-wait probe: elapsed time
   SubmitRing* ring = nullptr;       // subtree submissions (created on first use)
   uint32_t leaf_kernel = 1;         // 0: column-split kernel on CTA pairs where it applies, 1: one CTA per tile
-  uint32_t* async_err = nullptr;    // pinned, mapped error word of the calls that do not wait (created on first use)
+  uint32_t* async_err = nullptr;    // pinned, mapped error word of the calls that do not wait
   uint32_t* async_err_dev = nullptr;
 };
 
@@ -307,14 +307,24 @@ int clear_err(tessa_ctx* ctx, cudaStream_t st) {
   return TESSA_OK;
 }
 
+// The error word of the calls that do not wait.
+int make_async_word(tessa_ctx* ctx) {
+  void *p = nullptr, *d = nullptr;
+  CUDA_TRY(cudaHostAlloc(&p, 64, cudaHostAllocMapped));
+  memset(p, 0, 64);
+  ctx->async_err = static_cast<uint32_t*>(p);
+  CUDA_TRY(cudaHostGetDevicePointer(&d, p, 0));
+  ctx->async_err_dev = static_cast<uint32_t*>(d);
+  return TESSA_OK;
+}
+
 // Error bits that kernels of the calls that do not wait have left so far;
-// taking them clears the word.
+// taking them clears the word.  Threads may share the context: each bit is
+// taken by one of them.
 int take_async_error(tessa_ctx* ctx) {
-  if (!ctx->async_err) return TESSA_OK;
-  const uint32_t bits = *reinterpret_cast<volatile uint32_t*>(ctx->async_err);
-  if (bits == 0) return TESSA_OK;
-  *reinterpret_cast<volatile uint32_t*>(ctx->async_err) = 0;
-  return map_device_error(bits);
+  if (__atomic_load_n(ctx->async_err, __ATOMIC_RELAXED) == 0) return TESSA_OK;
+  const uint32_t bits = __atomic_exchange_n(ctx->async_err, 0u, __ATOMIC_ACQ_REL);
+  return bits ? map_device_error(bits) : TESSA_OK;
 }
 
 // Blocked scans: the inner loops have no early exit, so they vectorise.
@@ -768,18 +778,6 @@ int tessa::ctx_sm_count(const tessa_ctx* ctx) { return ctx->sm_count; }
 
 int tessa::async_begin(tessa_ctx* ctx, AsyncCtx* out) {
   TRY(bind(ctx));
-  if (!ctx->async_err) {
-    void* p = nullptr;
-    CUDA_TRY(cudaHostAlloc(&p, 64, cudaHostAllocMapped));
-    memset(p, 0, 64);
-    void* d = nullptr;
-    if (cudaError_t e = cudaHostGetDevicePointer(&d, p, 0)) {
-      cudaFreeHost(p);
-      return fail(TESSA_ERR_CUDA, "cudaHostGetDevicePointer: %s", cudaGetErrorString(e));
-    }
-    ctx->async_err = static_cast<uint32_t*>(p);
-    ctx->async_err_dev = static_cast<uint32_t*>(d);
-  }
   TRY(take_async_error(ctx));
   out->device = ctx->device;
   out->sm_count = ctx->sm_count;
@@ -838,6 +836,7 @@ int tessa_create(int device, tessa_ctx** out) {
     if (cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking) != cudaSuccess) r = fail(TESSA_ERR_CUDA, "stream create failed");
   }
   if (r == TESSA_OK) r = ctx->d_err.ensure(4);
+  if (r == TESSA_OK) r = make_async_word(ctx);
   if (r != TESSA_OK) {
     tessa_destroy(ctx);
     return r;
