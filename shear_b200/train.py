@@ -61,18 +61,25 @@ def _link(t):
     return t[:0].clone()
 
 
+# torch runs backwards on threads of its own, and ops.context() is a thread's:
+# each backward works on the context of its forward, so that what its kernels
+# report reaches the caller of the forward (ops.async_status()), and no context
+# is made inside a graph capture.
+
+
 class _Lookup(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, ids, scale):
+        out = ops.embedding_lookup(table, ids, scale)
         ctx.save_for_backward(ids)
-        ctx.rows, ctx.scale = table.shape[0], scale
-        return ops.embedding_lookup(table, ids, scale)
+        ctx.rows, ctx.scale, ctx.context = table.shape[0], scale, ops.context(out.get_device())
+        return out
 
     @staticmethod
     def backward(ctx, dout):
         (ids,) = ctx.saved_tensors
         d2 = _rows(dout.reshape(-1, dout.shape[-1]))
-        grad = ops.embedding_grad(d2, ids.reshape(-1), ctx.rows, ctx.scale)
+        grad = ops.embedding_grad(d2, ids.reshape(-1), ctx.rows, ctx.scale, ctx=ctx.context)
         return _first_order("lookup", grad, dout), None, None
 
 
@@ -84,7 +91,7 @@ class _ProductFp8(torch.autograd.Function):
         xc, xs, *x_t = ops.quantize_fp8_both(x) if need_w else ops.quantize_fp8(x)
         wc, ws, *w_t = ops.quantize_fp8_both(w) if need_x else ops.quantize_fp8(w)
         ctx.save_for_backward(*x_t, *w_t)
-        ctx.types, ctx.links = (x.dtype, w.dtype), links
+        ctx.types, ctx.links, ctx.context = (x.dtype, w.dtype), links, ops.context(x.get_device())
         return ops.matmul_fp8(xc, xs, wc, ws, out_dtype=out_dtype)
 
     @staticmethod
@@ -95,15 +102,15 @@ class _ProductFp8(torch.autograd.Function):
         dx = dw = None
         given, dy = dy, _rows(dy)
         if need_x and need_w:
-            c, s, ct, st = ops.quantize_fp8_both(dy)
+            c, s, ct, st = ops.quantize_fp8_both(dy, ctx=ctx.context)
         elif need_x:
-            c, s = ops.quantize_fp8(dy)
+            c, s = ops.quantize_fp8(dy, ctx=ctx.context)
         else:
-            ct, st = ops.quantize_fp8(dy, transpose=True)
+            ct, st = ops.quantize_fp8(dy, transpose=True, ctx=ctx.context)
         if need_x:
-            dx = ops.matmul_fp8(c, s, *saved, out_dtype=ctx.types[0])
+            dx = ops.matmul_fp8(c, s, *saved, out_dtype=ctx.types[0], ctx=ctx.context)
         if need_w:
-            dw = ops.matmul_fp8(ct, st, *x_t, out_dtype=ctx.types[1])
+            dw = ops.matmul_fp8(ct, st, *x_t, out_dtype=ctx.types[1], ctx=ctx.context)
         x, w = ctx.links
         return _first_order("product_fp8", dx, given, w), _first_order("product_fp8", dw, given, x), None, None
 
@@ -111,14 +118,15 @@ class _ProductFp8(torch.autograd.Function):
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher_ids, teacher_logits, temperature):
+        loss = ops.distill_topk(logits, teacher_ids, teacher_logits, temperature)[0]
         ctx.save_for_backward(logits, teacher_ids, teacher_logits)
-        ctx.temperature = temperature
-        return ops.distill_topk(logits, teacher_ids, teacher_logits, temperature)[0]
+        ctx.temperature, ctx.context = temperature, ops.context(loss.get_device())
+        return loss
 
     @staticmethod
     def backward(ctx, dloss):
         logits, ids, teacher = ctx.saved_tensors
-        grad = ops.distill_topk_grad(logits, ids, teacher, ctx.temperature, row_weights=dloss)[2]
+        grad = ops.distill_topk_grad(logits, ids, teacher, ctx.temperature, row_weights=dloss, ctx=ctx.context)[2]
         return _first_order("distill", grad, dloss, logits), None, None, None
 
 

@@ -1,5 +1,7 @@
 """The trainer and the differentiable functions with plain torch in place of
 the kernels, so that they run without a GPU."""
+import threading
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -57,7 +59,14 @@ def train(monkeypatch):
              "distill_topk_grad": _distill, "distill_topk": lambda *a, **k: _distill(*a, **k)[:2]}
     for name, f in plain.items():
         monkeypatch.setattr(train.ops, name, torch.no_grad()(f))  # as kernels do, they leave no graph
-    return train
+    seen = []  # (operator, context)
+    for name in plain:
+        f = getattr(train.ops, name)
+        monkeypatch.setattr(train.ops, name, lambda *a, _f=f, _n=name, **k: (seen.append((_n, k.get("ctx"))), _f(*a, **k))[1])
+    monkeypatch.setattr(train.ops, "context", lambda device=0: f"context of {threading.current_thread().name}")
+    train.seen = seen
+    yield train
+    del train.seen
 
 
 def _trainer(train, rows=12, dim=5):
@@ -150,3 +159,15 @@ def test_a_second_derivative_past_these_functions(train):
     y.backward(create_graph=True)
     gv.sum().backward()
     assert torch.equal(v.grad.detach(), 2 * v.detach() + 2)
+
+
+def test_backwards_use_the_context_of_their_forward(train):
+    # as torch does on a GPU: the backward on another thread
+    for _, f, tensors in _first_order_cases(train):
+        y = f(*(t.requires_grad_() for t in tensors))
+        del train.seen[:]
+        backward = threading.Thread(target=y.backward, name="backward")
+        backward.start()
+        backward.join()
+        here = f"context of {threading.current_thread().name}"
+        assert train.seen and all(used == here for _, used in train.seen), train.seen

@@ -47,3 +47,53 @@ def test_threads_share_a_context():
         codes.append(lib.tessa_async_status(ctx.handle, None))
         assert len(codes) == 17 and sorted(codes) == [-5] + [0] * 16, (turn, codes)
         ctx.close()
+
+
+@pytest.mark.parametrize("name", ["lookup", "distill"])
+def test_an_error_in_a_backward_reaches_the_caller(name):
+    import torch
+    from shear_b200 import ops, train
+    from shear_b200._capi import TessaError
+    t = torch.randn(20, 30, device="cuda").requires_grad_()
+    ids = torch.randint(0, 20, (20, 3), device="cuda")
+    y = train.lookup(t, ids) if name == "lookup" else train.distill(t, ids, torch.randn(20, 3, device="cuda"))
+    ops.async_status()
+    ids.data[4, 1] = 30  # between the two
+    y.sum().backward()
+    with pytest.raises(TessaError) as e:
+        ops.async_status()
+    assert e.value.code == -5
+    ops.async_status()
+
+
+CAPTURE = """
+import torch
+from shear_b200 import ops, train
+g = torch.Generator().manual_seed(0)
+rand = lambda *s: torch.randn(*s, generator=g).cuda().requires_grad_()
+table, x, w, z = rand(50, 32), rand(40, 64), rand(30, 64), rand(8, 90)
+ids, lists, teacher = (torch.randint(0, 50, (20,), generator=g).cuda(), torch.randint(0, 90, (8, 4), generator=g).cuda(),
+                       torch.randn(8, 4, generator=g).cuda())
+def forward():
+    return train.lookup(table, ids).sum(), train.product_fp8(x, w).sum(), train.distill(z, lists, teacher).sum()
+def backward(y):
+    return torch.autograd.grad(y, (table, x, w, z))
+side = torch.cuda.Stream()
+with torch.cuda.stream(side):
+    forward()  # no backward has run when the capture begins
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        grads = backward(sum(forward()))
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(grads, backward(sum(forward()))):
+        assert torch.equal(a, b) and a.abs().sum() > 0
+ops.async_status()
+print("same")
+"""
+
+
+def test_a_first_backward_inside_a_capture():
+    run = subprocess.run([sys.executable, "-c", CAPTURE], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.strip() == "same", run.stderr[-2000:]
