@@ -868,6 +868,12 @@ def _workspace(nbytes: int, device):
     return _torch.empty_strided((nbytes,), (1,), dtype=_torch.uint8, device=device) if nbytes else None
 
 
+def _written(out):
+    """`out` holds other values now: a graph that saved it must find out, as after torch's own writes."""
+    if not out.is_inference():
+        _torch.autograd.graph.increment_version(out)
+
+
 def async_status(ctx: Context | None = None, device: int = 0) -> None:
     """Waits for the current stream and raises what the calls of this section left (tessa_async_status)."""
     _lazy_torch()
@@ -902,6 +908,8 @@ def embedding_lookup(table, ids, scale: float = 1.0, out=None, out_dtype=None, c
     a = C.LookupArgs(table.data_ptr(), rows, stride, dim, code, flat.data_ptr(), id_bits, out_code, n, scale,
                      res.data_ptr(), out_stride)
     C.check(C.load().tessa_embedding_lookup((ctx or context(dev)).handle, a, _stream(dev)))
+    if out is not None:
+        _written(out)
     return res
 
 
@@ -930,22 +938,25 @@ def embedding_grad(dout, ids, table_rows: int, scale: float = 1.0, out_dtype=Non
         raise ValueError("accumulate needs out")
     if out is None:
         out_stride, out_code = dim, code if out_dtype is None else _dtype_code("out", out_dtype)
-        out = _empty(table_rows, dim, out_dtype or dout.dtype, dout.device)
+        grad = _empty(table_rows, dim, out_dtype or dout.dtype, dout.device)
     else:
         if tuple(out.shape) != (table_rows, dim):
             raise ValueError(f"out has shape {tuple(out.shape)}, not {(table_rows, dim)}")
         if out_dtype is not None and out.dtype != out_dtype:
             raise ValueError(f"out is {out.dtype}, not {out_dtype}")
         _, _, out_stride, out_code = _matrix("out", out, dev)
+        grad = out
     lib = C.load()
     need = ctypes.c_uint64()
     C.check(lib.tessa_embedding_grad_workspace(n, table_rows, dim, need))
     ws = _workspace(need.value, dout.device)
     a = C.LookupGradArgs(d2.data_ptr(), stride, dim, code, flat.data_ptr(), id_bits, out_code, n, scale,
-                         1 if accumulate else 0, out.data_ptr(), out_stride, table_rows)
+                         1 if accumulate else 0, grad.data_ptr(), out_stride, table_rows)
     C.check(lib.tessa_embedding_grad((ctx or context(dev)).handle, a, ws.data_ptr() if ws is not None else None,
                                      need.value, _stream(dev)))
-    return out
+    if out is not None:
+        _written(out)
+    return grad
 
 
 def _fp8_shape(rows: int, cols: int):
@@ -1018,20 +1029,23 @@ def matmul_fp8(a_codes, a_scales, b_codes, b_scales, out_dtype=None, out=None, c
                          f"{b_codes.device}")
     if out is None:
         out_stride, out_code = n, 0 if out_dtype is None else _dtype_code("out", out_dtype)
-        out = _empty(m, n, out_dtype or torch.float32, a_codes.device)
+        res = _empty(m, n, out_dtype or torch.float32, a_codes.device)
     else:
         if tuple(out.shape) != (m, n) or (out_dtype is not None and out.dtype != out_dtype):
             raise ValueError(f"out must be {(m, n)}" + (f" of {out_dtype}" if out_dtype is not None else ""))
         _, _, out_stride, out_code = _matrix("out", out, dev)
+        res = out
     lib = C.load()
     handle = (ctx or context(dev)).handle
     need = ctypes.c_uint64()
     C.check(lib.tessa_matmul_fp8_workspace(handle, m, n, k, need))
     ws = _workspace(need.value, a_codes.device)
     a = C.Fp8MatmulArgs(a_codes.data_ptr(), a_scales.data_ptr(), b_codes.data_ptr(), b_scales.data_ptr(), m, n, k,
-                        out.data_ptr(), out_stride, out_code, 0)
+                        res.data_ptr(), out_stride, out_code, 0)
     C.check(lib.tessa_matmul_fp8(handle, a, ws.data_ptr() if ws is not None else None, need.value, _stream(dev)))
-    return out
+    if out is not None:
+        _written(out)
+    return res
 
 
 def _distill(logits, teacher_ids, teacher_logits, temperature, row_weights, want_grad, out, ctx):
@@ -1071,6 +1085,8 @@ def _distill(logits, teacher_ids, teacher_logits, temperature, row_weights, want
         ws = _workspace(need.value, device)
     C.check(lib.tessa_distill_topk((ctx or context(dev)).handle, a, ws.data_ptr() if ws is not None else None,
                                    need.value, _stream(dev)))
+    if out is not None:
+        _written(out)
     return loss, lse, grad
 
 
