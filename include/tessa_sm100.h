@@ -797,7 +797,8 @@ TESSA_API int tessa_matmul_fp8(tessa_ctx* ctx, const tessa_fp8_matmul_args* args
  * all -inf, takes no part: loss 0, gradient 0.  An entry whose logit is -inf
  * while others are not makes the loss +inf, as the formula says.
  * grad may be NULL (loss alone); it may be logits itself (same type and
- * stride).  Statistics and sums in f32; grad rounded once to the logits' type. */
+ * stride), but not overlap it otherwise (TESSA_ERR_INVALID_ARG).  Statistics
+ * and sums in f32; grad rounded once to the logits' type. */
 #define TESSA_MAX_DISTILL_K 1024
 typedef struct tessa_distill_args {
   const void* logits;           /* rows x vocab */

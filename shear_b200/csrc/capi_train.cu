@@ -63,6 +63,27 @@ int check_workspace(const void* ws, uint64_t have, uint64_t need) {
   return TESSA_OK;
 }
 
+// Whether any row at p (`bytes` long, p_step from one to the next) shares memory
+// with a row at q, other than being all of the same row.
+bool rows_overlap(const void* p, uint64_t p_step, const void* q, uint64_t q_step, uint64_t rows, uint64_t bytes) {
+  if (rows == 0 || bytes == 0) return false;
+  const uint64_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q), last = rows - 1;
+  if (a + last * p_step + bytes <= b || b + last * q_step + bytes <= a) return false;
+  if (a == b && (rows == 1 || p_step == q_step)) return false;
+  if (rows == 1) return true;
+  if (p_step == q_step) {  // side by side in one wider matrix, or not
+    const uint64_t d = (a < b ? b - a : a - b) % p_step;
+    return d < bytes || p_step - d < bytes;
+  }
+  for (uint64_t i = 0, j = 0; i < rows && j < rows;) {
+    const uint64_t x = a + i * p_step, y = b + j * q_step;
+    if (x + bytes <= y) ++i;
+    else if (y + bytes <= x) ++j;
+    else return true;
+  }
+  return false;
+}
+
 int launched(const char* what, cudaError_t e) {
   if (e == cudaSuccess) return TESSA_OK;
   return bad(e == cudaErrorMemoryAllocation ? TESSA_ERR_OOM : TESSA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
@@ -188,6 +209,9 @@ int tessa_distill_topk(tessa_ctx* ctx, const tessa_distill_args* args, void* wor
   if (a.grad) TRY(check_matrix("grad", a.grad, a.rows, a.vocab, a.grad_stride, a.dtype));
   if (a.grad == a.logits && a.rows > 1 && a.grad_stride != a.stride)
     return bad(TESSA_ERR_INVALID_ARG, "a gradient in place of the logits needs their stride");
+  const uint64_t bytes = elem_bytes(a.dtype);
+  if (a.grad && rows_overlap(a.logits, a.stride * bytes, a.grad, a.grad_stride * bytes, a.rows, a.vocab * bytes))
+    return bad(TESSA_ERR_INVALID_ARG, "the gradient overlaps the logits: it may be in their place, or apart");
   if (a.k > TESSA_MAX_DISTILL_K) return bad(TESSA_ERR_INVALID_ARG, "list of %u entries: at most %d", a.k, TESSA_MAX_DISTILL_K);
   if (a.vocab > kMaxTableRows) return bad(TESSA_ERR_UNSUPPORTED, "%llu logits a row", (ull)a.vocab);
   if (a.rows > (1ull << 27)) return bad(TESSA_ERR_UNSUPPORTED, "%llu rows: at most 2^27", (ull)a.rows);

@@ -1109,6 +1109,7 @@ def distill_topk_grad(logits, teacher_ids, teacher_logits, temperature: float = 
     of sum(row_weights * loss) with respect to them.
 
     Returns (loss, lse, grad [rows, vocab] in the logits' type).  out receives
-    the gradient; it may be the logits themselves.
+    the gradient; it may be the logits themselves, but not overlap them
+    otherwise.
     """
     return _distill(logits, teacher_ids, teacher_logits, temperature, row_weights, True, out, ctx)

@@ -34,3 +34,44 @@ def test_a_graph_that_saved_the_output_finds_it_written(name):
         call(z.normal_())
     call(z)  # (an inference tensor counts no versions)
     ops.async_status()
+
+
+def _strided(torch, flat, rows, cols, step, at):
+    return torch.as_strided(flat, (rows, cols), (step, 1), at)
+
+
+@pytest.mark.parametrize("rows,logits,out", [  # (row stride, first element) of rows of 100
+    (6, (100, 0), (100, 100)), (6, (100, 100), (100, 0)),    # one row on, one row back
+    (6, (200, 0), (200, 50)), (6, (200, 150), (200, 0)),     # columns in common, or the neighbour's
+    (1, (100, 0), (100, 99)), (2, (300, 0), (300, 399)),     # one element
+    (4, (200, 0), (400, 350)), (4, (150, 500), (1000, 0)),   # strides that meet later
+])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_gradient_that_overlaps_the_logits_is_refused(rows, logits, out, dtype):
+    import torch
+    from shear_b200 import ops
+    from shear_b200._capi import TessaError
+    flat = torch.randn(8000, device="cuda").to(getattr(torch, dtype))
+    before = flat.clone()
+    ids, t = torch.randint(0, 100, (rows, 3), device="cuda"), torch.randn(rows, 3, device="cuda")
+    with pytest.raises(TessaError) as e:
+        ops.distill_topk_grad(_strided(torch, flat, rows, 100, *logits), ids, t, out=_strided(torch, flat, rows, 100, *out))
+    assert e.value.code == -1 and torch.equal(flat, before)
+
+
+@pytest.mark.parametrize("rows,logits,out", [
+    (6, (200, 0), (200, 100)), (6, (200, 100), (200, 0)),    # side by side
+    (6, (201, 0), (201, 101)), (1, (100, 0), (100, 100)), (3, (100, 0), (100, 300)),
+    (3, (400, 0), (200, 100)), (2, (1000, 300), (500, 0)),   # in each other's gaps
+    (6, (200, 0), (200, 0)),                                 # in place
+])
+def test_a_gradient_beside_the_logits(rows, logits, out):
+    import torch
+    from shear_b200 import ops
+    flat = torch.randn(8000, device="cuda")
+    ids, t = torch.randint(0, 100, (rows, 3), device="cuda"), torch.randn(rows, 3, device="cuda")
+    z = _strided(torch, flat, rows, 100, *logits)
+    want = ops.distill_topk_grad(z, ids, t)
+    got = ops.distill_topk_grad(z, ids, t, out=_strided(torch, flat, rows, 100, *out))
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
