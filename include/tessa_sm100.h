@@ -688,6 +688,7 @@ TESSA_API void tessa_replay_session_destroy(tessa_replay_session* session);
  * which waits for `stream` first; either report clears it.  Unlike all others,
  * these calls and tessa_async_status may be made on one context by several host
  * threads at once; each error is then reported to one of them.
+ * They leave the calling thread's current device as it was.
  * A bad id is never read through: its row counts as padding.
  *
  * Matrices are row-major device memory with `stride` elements from row to row

@@ -777,7 +777,7 @@ int assign_device(tessa_ctx* ctx, uint32_t source, const tessa_assign_args* a, c
 int tessa::ctx_sm_count(const tessa_ctx* ctx) { return ctx->sm_count; }
 
 int tessa::async_begin(tessa_ctx* ctx, AsyncCtx* out) {
-  TRY(bind(ctx));
+  CUDA_TRY((cudaError_t)out->scope.enter(ctx->device));
   TRY(take_async_error(ctx));
   out->device = ctx->device;
   out->sm_count = ctx->sm_count;
@@ -789,7 +789,9 @@ int tessa::async_begin(tessa_ctx* ctx, AsyncCtx* out) {
 extern "C" {
 
 int tessa_async_status(tessa_ctx* ctx, void* stream) {
-  TRY(bind(ctx));
+  if (!ctx) return fail(TESSA_ERR_INVALID_ARG, "null context");
+  DeviceScope<CudaDevices> scope;
+  CUDA_TRY((cudaError_t)scope.enter(ctx->device));
   CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
   return take_async_error(ctx);
 }
@@ -831,7 +833,8 @@ int tessa_create(int device, tessa_ctx** out) {
   if (!ctx) return fail(TESSA_ERR_OOM, "context allocation failed");
   ctx->device = device;
   ctx->sm_count = prop.multiProcessorCount;
-  int r = bind(ctx);
+  DeviceScope<CudaDevices> scope;
+  int r = scope.enter(device) == 0 ? TESSA_OK : fail(TESSA_ERR_CUDA, "device %d cannot be made current", device);
   if (r == TESSA_OK) {
     if (cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking) != cudaSuccess) r = fail(TESSA_ERR_CUDA, "stream create failed");
   }
@@ -847,9 +850,10 @@ int tessa_create(int device, tessa_ctx** out) {
 
 void tessa_destroy(tessa_ctx* ctx) {
   if (!ctx) return;
+  DeviceScope<CudaDevices> scope;
+  scope.enter(ctx->device);
   submit_ring_destroy(ctx->ring);  // waits for queued submissions
   ctx->ring = nullptr;
-  cudaSetDevice(ctx->device);
   if (ctx->stream) cudaStreamSynchronize(ctx->stream);
   ctx->d_err.release();
   ctx->gather.release();

@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include "../../include/tessa_sm100.h"
+#include "device_scope.h"
 
 namespace tessa {
 
@@ -236,10 +237,17 @@ int submit_ring_poll(SubmitRing* ring, uint64_t ticket, int wait, tessa_compact_
 int submit_ring_release(SubmitRing* ring, uint64_t ticket);
 size_t reservoir_scratch_bytes(uint64_t edges, uint64_t num_points);
 
+struct CudaDevices {
+  static int get(int* device) { return (int)cudaGetDevice(device); }
+  static int set(int device) { return (int)cudaSetDevice(device); }
+};
+
 // What the calls that only enqueue work need from a context: async_begin
-// binds its device and reports what an earlier call's kernel left in the
-// mapped error word `err`.
+// makes its device current until the AsyncCtx goes (the caller may stand between
+// operators of another library that go by the current device) and reports what an
+// earlier call's kernel left in the mapped error word `err`.
 struct AsyncCtx {
+  DeviceScope<CudaDevices> scope;
   int device;
   int sm_count;
   uint64_t timeout_ns;
