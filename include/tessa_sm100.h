@@ -769,7 +769,9 @@ TESSA_API int tessa_quantize_fp8(tessa_ctx* ctx, const tessa_fp8_quantize_args* 
 
 /* out[m][n] = sum over blocks of sa * sb * (a . b): a is m x k codes, b n x k
  * codes in the layout above (k a multiple of 16), products summed in f32 on
- * the tensor cores and rounded once to out's type. */
+ * the tensor cores and rounded once to out's type.  m, n and k are below 2^31;
+ * a product of 2^31 tiles and more (a tile is at most 256 x 224 outputs, and at
+ * most 8192 of k) is TESSA_ERR_UNSUPPORTED. */
 typedef struct tessa_fp8_matmul_args {
   const uint8_t* a_codes;
   const uint8_t* a_scales;

@@ -178,7 +178,7 @@ int tessa_matmul_fp8(tessa_ctx* ctx, const tessa_fp8_matmul_args* args, void* wo
   uint64_t need = 0;
   TRY(tessa_matmul_fp8_workspace(ctx, a.m, a.n, a.k, &need));
   if (a.k % 16) return bad(TESSA_ERR_INVALID_ARG, "k=%llu: rows of codes are a multiple of 16", (ull)a.k);
-  if ((a.m + 15) / 16 * ((a.n + 127) / 128) > kMaxMatrix / 32)
+  if (fp8_matmul_units(a.m, a.n, a.k, ctx_sm_count(ctx)) > kMaxMatrix)
     return bad(TESSA_ERR_UNSUPPORTED, "product of %llu x %llu is too large", (ull)a.m, (ull)a.n);
   if (a.m && a.n && a.k) {
     if (!a.a_codes || !a.a_scales || !a.b_codes || !a.b_scales) return bad(TESSA_ERR_INVALID_ARG, "null codes or scales");

@@ -700,6 +700,17 @@ uint64_t fp8_matmul_workspace(uint64_t m, uint64_t n, uint64_t k, int sm_count) 
   return splits > 1 ? (uint64_t)splits * m * div_up(n, 4) * 16 : 0;
 }
 
+uint64_t fp8_matmul_units(uint64_t m, uint64_t n, uint64_t k, int sm_count) {
+  using namespace train;
+  if (m == 0 || n == 0 || k == 0 || few_rows(m, n)) return 0;
+  auto units = [&](uint64_t rows_p, uint64_t rows_q) {
+    const mm::Plan p = mm::plan_of(rows_p, rows_q, k, sm_count);
+    return (uint64_t)p.tiles_p * p.tiles_q * p.splits;
+  };
+  const uint64_t one = units(m, n), other = units(n, m);  // which of the two depends on out's alignment
+  return one > other ? one : other;
+}
+
 cudaError_t launch_matmul_fp8(const tessa_fp8_matmul_args& a, void* workspace, const AsyncCtx& c,
                               cudaStream_t stream) {
   using namespace train;

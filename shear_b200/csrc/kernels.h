@@ -264,6 +264,8 @@ cudaError_t launch_embedding_grad(const tessa_lookup_grad_args& a, void* workspa
                                   cudaStream_t stream);
 cudaError_t launch_quantize_fp8(const tessa_fp8_quantize_args& a, const AsyncCtx& c, cudaStream_t stream);
 uint64_t fp8_matmul_workspace(uint64_t m, uint64_t n, uint64_t k, int sm_count);
+// Tiles times splits of K of a product, which the kernel counts in 32 bits.
+uint64_t fp8_matmul_units(uint64_t m, uint64_t n, uint64_t k, int sm_count);
 cudaError_t launch_matmul_fp8(const tessa_fp8_matmul_args& a, void* workspace, const AsyncCtx& c,
                               cudaStream_t stream);
 cudaError_t launch_fp8_few_rows(const tessa_fp8_matmul_args& a, const AsyncCtx& c, cudaStream_t stream);

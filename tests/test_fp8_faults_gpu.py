@@ -22,3 +22,42 @@ def test_a_product_longer_than_the_wait_limit():
     ops.async_status(ctx)
     assert times[0].elapsed_time(times[1]) > 15.0  # 70 TFLOP, so that the test is one
     assert (out == 8192).all()
+
+
+@pytest.mark.parametrize("n", [1, 9, 16])
+def test_a_billion_rows(n):
+    # few columns: read in registers, and by tiles either way round (rows of 18 bytes do not suit TMA)
+    import torch
+    from shear_b200 import ops
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 64 << 30:
+        pytest.skip("needs 64 GiB of device memory")
+    m, width = 1_090_000_000, 16
+    a = torch.full((m, width), 0x38, dtype=torch.uint8, device="cuda")       # ones
+    s = torch.full((m, 4), 127, dtype=torch.uint8, device="cuda")
+    marks = [0, 1, 255, 256, m // 2, 2 ** 30 - 1, 2 ** 30, m - 257, m - 1]
+    for i, r in enumerate(marks):
+        a[r] = 0x40                                                          # twos
+        s[r, 0] = 127 + i
+    b = torch.full((n, width), 0x38, dtype=torch.uint8, device="cuda")
+    t = torch.full((n, 4), 127, dtype=torch.uint8, device="cuda")
+    t[:, 0] += torch.arange(n, device="cuda", dtype=torch.uint8) % 4         # column j times 2^(j % 4)
+    out = ops.matmul_fp8(a, s, b, t, out_dtype=torch.bfloat16)
+    ops.async_status()
+    column = 2.0 ** (torch.arange(n, device="cuda") % 4)
+    want = torch.tensor([32.0 * 2.0 ** i for i in range(len(marks))], device="cuda")[:, None] * column
+    assert torch.equal(out[marks].float(), want)
+    out[marks] = (16.0 * column).bfloat16()
+    for first in range(0, m, 1 << 26):
+        assert (out[first: first + (1 << 26)] == (16.0 * column).bfloat16()).all()
+
+
+def test_products_of_too_many_tiles_are_refused():
+    # before any launch: the operands are not there
+    import torch
+    from shear_b200 import _capi as C, ops
+    lib, h = C.load(), ops.context(0).handle
+    p = torch.zeros(256, device="cuda").data_ptr()
+    most = 2 ** 31 - 1
+    assert lib.tessa_matmul_fp8(h, C.Fp8MatmulArgs(p, p, p, p, most, most, 16, p, most, 1, 0), None, 0, None) == -6
+    assert lib.tessa_matmul_fp8(h, C.Fp8MatmulArgs(p, p, p, p, 2 ** 31, 1, 16, p, 1, 1, 0), None, 0, None) == -6
