@@ -219,6 +219,8 @@ int tessa_distill_topk(tessa_ctx* ctx, const tessa_distill_args* args, void* wor
   if (a.rows * a.k && !a.teacher_logits) return bad(TESSA_ERR_INVALID_ARG, "teacher logits: null pointer");
   if (!(a.temperature > 0.0f) || a.temperature > 3.0e38f)
     return bad(TESSA_ERR_INVALID_ARG, "temperature %g: a positive number", (double)a.temperature);
+  if (1.44269504f / a.temperature > 3.402823466e38f)  // log2(e) / tau is a factor: infinite, it makes 0 * inf of equal logits
+    return bad(TESSA_ERR_INVALID_ARG, "temperature %g: at least 4.24e-39", (double)a.temperature);
   TRY(check_workspace(workspace, workspace_bytes, distill_workspace(a.rows, a.vocab, a.dtype, a.k, a.grad != nullptr)));
   AsyncCtx c;
   TRY(async_begin(ctx, &c));

@@ -75,3 +75,21 @@ def test_a_gradient_beside_the_logits(rows, logits, out):
     got = ops.distill_topk_grad(z, ids, t, out=_strided(torch, flat, rows, 100, *out))
     for x, y in zip(got, want):
         assert torch.equal(x, y)
+
+
+def test_the_least_temperatures():
+    # all weight on the largest logit, in list and row, or a refusal; never NaN
+    import torch
+    from shear_b200 import ops
+    from shear_b200._capi import TessaError
+    z, t = torch.tensor([[0.5, 1.0, -1.0, 1.0]], device="cuda"), torch.tensor([[0.25, 1.0]], device="cuda")
+    ids = torch.tensor([[1, 0]], device="cuda")
+    for tau in (1e-38, 4.3e-39):
+        _, lse, grad = ops.distill_topk_grad(z, ids, t, tau, row_weights=torch.full((1,), 1e37, device="cuda"))
+        scale = float(torch.tensor(tau).double()) * float(torch.tensor(1e37).double())
+        want = torch.tensor([[-scale, scale / 2, 0.0, scale / 2]], device="cuda")
+        assert torch.allclose(grad, want, rtol=1e-5, atol=0) and lse.isfinite().all()
+    for tau in (4.2e-39, 1e-40, 1e-45):
+        with pytest.raises(TessaError) as e:
+            ops.distill_topk_grad(z, ids, t, tau)
+        assert e.value.code == -1
