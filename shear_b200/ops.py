@@ -850,6 +850,11 @@ def _matrix(name: str, t, dev=None):
     return rows, cols, step, _dtype_code(name, t.dtype)
 
 
+def _as_rows(t):
+    """t as a matrix of its last axis (also where that has no elements)."""
+    return t if t.dim() == 2 else t.flatten(0, -2) if t.dim() > 2 else t.unsqueeze(0)
+
+
 def _empty(rows: int, cols: int, dtype, device):
     return _torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
 
@@ -926,7 +931,7 @@ def embedding_grad(dout, ids, table_rows: int, scale: float = 1.0, out_dtype=Non
     names as they are.
     """
     torch = _lazy_torch()
-    d2 = dout if dout.dim() == 2 else dout.reshape(-1, dout.shape[-1])
+    d2 = _as_rows(dout)
     d_rows, dim, stride, code = _matrix("dout", d2)
     dev = d2.get_device()
     flat, id_bits = _id_tensor(ids, dev)

@@ -78,8 +78,7 @@ class _Lookup(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         (ids,) = ctx.saved_tensors
-        d2 = _rows(dout.reshape(-1, dout.shape[-1]))
-        grad = ops.embedding_grad(d2, ids.reshape(-1), ctx.rows, ctx.scale, ctx=ctx.context)
+        grad = ops.embedding_grad(_rows(ops._as_rows(dout)), ids.reshape(-1), ctx.rows, ctx.scale, ctx=ctx.context)
         return _first_order("lookup", grad, dout), None, None
 
 

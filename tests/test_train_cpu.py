@@ -171,3 +171,12 @@ def test_backwards_use_the_context_of_their_forward(train):
         backward.join()
         here = f"context of {threading.current_thread().name}"
         assert train.seen and all(used == here for _, used in train.seen), train.seen
+
+
+@pytest.mark.parametrize("shape", [(), (3,), (0,), (2, 3), (2, 0, 3)])
+@pytest.mark.parametrize("dim", [0, 1, 4])
+def test_lookups_of_any_shape(train, shape, dim):
+    t = torch.randn(5, dim).requires_grad_()
+    ids = torch.randint(0, 5, shape)
+    train.lookup(t, ids).sum().backward()
+    assert torch.equal(t.grad, torch.bincount(ids.reshape(-1), minlength=5)[:, None].expand(5, dim).float())

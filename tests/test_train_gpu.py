@@ -255,3 +255,19 @@ def test_second_derivatives_are_refused(name):
     assert torch.equal(g.detach(), plain)
     with pytest.raises(RuntimeError, match=f"{name} has no second derivative"):
         torch.autograd.grad(g.square().sum() + t.sum() + w.sum(), w if name == "product_fp8" else t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(), (3,), (0,), (2, 3), (2, 0, 3)])
+@pytest.mark.parametrize("dim", [0, 1, 4])
+def test_lookups_of_any_shape(shape, dim):
+    import torch
+    from shear_b200 import ops, train
+    t = torch.randn(5, dim, device="cuda").requires_grad_()
+    ids = torch.randint(0, 5, shape, device="cuda")
+    y = train.lookup(t, ids)
+    assert y.shape == (*shape, dim)
+    y.sum().backward()
+    want = torch.bincount(ids.reshape(-1), minlength=5)[:, None].expand(5, dim).float()
+    assert torch.equal(t.grad, want)
+    assert torch.equal(ops.embedding_grad(torch.ones(*shape, dim, device="cuda"), ids, 5), want)
