@@ -61,3 +61,26 @@ def test_products_of_too_many_tiles_are_refused():
     most = 2 ** 31 - 1
     assert lib.tessa_matmul_fp8(h, C.Fp8MatmulArgs(p, p, p, p, most, most, 16, p, most, 1, 0), None, 0, None) == -6
     assert lib.tessa_matmul_fp8(h, C.Fp8MatmulArgs(p, p, p, p, 2 ** 31, 1, 16, p, 1, 1, 0), None, 0, None) == -6
+
+
+@pytest.mark.parametrize("m,n", [(130, 300), (16, 40), (1, 300), (7, 5)])
+@pytest.mark.parametrize("k", [4096, 8192, 40_000, 131_072])
+def test_long_sums_of_one_sign(m, n, k):
+    # An f32 accumulator that is cut towards zero loses up to 2^-23 of itself a
+    # step of 32 terms, and with terms of one sign it grows evenly: half of that
+    # a step, of the whole.  Parts of at most 8192 terms, 256 steps, keep that
+    # from growing with k; within a step 33 terms are held to 24 bits of the
+    # largest, and parts are added with rounding.  With few rows on one side
+    # blocks of 128 are added with rounding, half of 2^-24 of the whole each.
+    import torch
+    from shear_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(k + m)
+    codes = [torch.randint(0x30, 0x48, (r, k), generator=g, device="cuda").to(torch.uint8) for r in (m, n)]
+    scales = [torch.full((r, -(-k // 512) * 4), 127, dtype=torch.uint8, device="cuda") for r in (m, n)]
+    got = ops.matmul_fp8(codes[0], scales[0], codes[1], scales[1])
+    ops.async_status()
+    a, b = (c.view(torch.float8_e4m3fn).double() for c in codes)
+    want = a @ b.t()
+    few = min(m, n) <= 8
+    steps = -(-k // 128) / 2 * 2.0 ** -24 + 5 * 2.0 ** -23 if few else 257 / 2 * 2.0 ** -23 + -(-k // 8192) * 2.0 ** -24
+    assert ((got.double() - want).abs() <= (steps + 33 * 2.0 ** -24) * want).all(), float(((got - want) / want).abs().max())
