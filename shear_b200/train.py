@@ -57,8 +57,8 @@ def _first_order(name, grad, *depends):
 
 
 def _link(t):
-    """An empty tensor that depends on t without holding its memory."""
-    return t[:0].clone()
+    """What depends on the matrix t without holding memory that the graph does not hold anyway."""
+    return t if t.is_leaf else t.repeat(0, 1)
 
 
 # torch runs backwards on threads of its own, and ops.context() is a thread's:
@@ -182,28 +182,34 @@ class TableTrainer:
         if not temperature > 0:
             raise ValueError("temperature must be positive")
         self.table, self.rate, self.temperature, self.scale = table, rate, temperature, scale
+        self._no_entry = torch.full((), -1, dtype=torch.int32, device=table.device)
 
     def _named(self, ids):
-        """Which ids name a row of the table."""
-        return (ids >= 0) & (ids < self.table.shape[0])
+        """(ids brought into the table, which of them name a row of it)."""
+        rows = self.table.shape[0]
+        inside = ids.clamp(0, max(rows - 1, 0))
+        return inside, inside == ids if rows else torch.zeros_like(ids, dtype=torch.bool)
 
     def scores(self, ids):
         """scale * table[ids] . table^T in bf16, each row's own score -inf; and the codes that its gradient needs."""
+        return self._scores(ids, self._named(ids)[0])
+
+    def _scores(self, ids, inside):
         x = ops.embedding_lookup(self.table, ids, self.scale)
         xq, wq = ops.quantize_fp8_both(x), ops.quantize_fp8_both(self.table)
         z = ops.matmul_fp8(*xq[:2], *wq[:2], out_dtype=torch.bfloat16)
         if z.shape[1]:  # (the row of an id outside the table takes no part, whichever of its scores this hides)
-            z.scatter_(1, ids.long().clamp(0, z.shape[1] - 1).unsqueeze(1), float("-inf"))
+            z.scatter_(1, inside.long().unsqueeze(1), float("-inf"))
         return z, xq[2:], wq[2:]
 
     def step(self, ids, teacher_ids, teacher_logits):
         """One step on the batch; returns its mean loss (a device scalar).  Rows of id -1 take
         no part, nor do those of an id outside the table, which the next call reports."""
-        z, x_t, w_t = self.scores(ids)
-        named = self._named(ids)
+        inside, named = self._named(ids)
+        z, x_t, w_t = self._scores(ids, inside)
         # a padding row's list may hold anything, an entry of the hidden score among
         # it, of which the loss is infinite: only without entries it takes no part
-        teacher_ids = teacher_ids.masked_fill(~named.unsqueeze(1), -1)
+        teacher_ids = torch.where(named.unsqueeze(1), teacher_ids, self._no_entry)
         weights = named.float()
         weights /= weights.sum().clamp(min=1.0)
         loss, _, dz = ops.distill_topk_grad(z, teacher_ids, teacher_logits, self.temperature, weights, out=z)
@@ -216,8 +222,9 @@ class TableTrainer:
 
     def recall(self, ids, teacher_ids) -> float:
         """Share of the teacher's neighbours of these rows among the table's own first k."""
-        z = self.scores(ids)[0]
-        teacher_ids = teacher_ids.masked_fill(~self._named(ids).unsqueeze(1), -1)
+        inside, named = self._named(ids)
+        z = self._scores(ids, inside)[0]
+        teacher_ids = torch.where(named.unsqueeze(1), teacher_ids, self._no_entry)
         got = z.topk(teacher_ids.shape[1], dim=1).indices.int()
         hit = (got.unsqueeze(2) == teacher_ids.unsqueeze(1)).any(1) & (teacher_ids >= 0)
         return float(hit.sum() / (teacher_ids >= 0).sum().clamp(min=1))

@@ -126,13 +126,14 @@ def _first_order_cases(train):
     return [
         ("lookup", lambda t: train.lookup(t, ids).pow(3).sum(), (rand(4, 5),)),
         ("product_fp8", lambda x, w: train.product_fp8(x, w).sum(), (rand(3, 4), rand(5, 4))),
+        ("product_fp8", lambda x, w: train.product_fp8(2 * x, -w).sum(), (rand(3, 4), rand(5, 4))),
         ("product_fp8", lambda x: train.product_fp8(x, torch.ones(2, 4)).square().sum(), (rand(3, 4),)),
         ("product_fp8", lambda w: train.product_fp8(torch.ones(2, 4), w).square().sum(), (rand(3, 4),)),
         ("distill", lambda z: train.distill(z, lists, torch.ones(3, 2), 1.5).sum(), (rand(3, 5),)),
     ]
 
 
-@pytest.mark.parametrize("case", range(5))
+@pytest.mark.parametrize("case", range(6))
 def test_a_second_derivative_is_refused_not_lost(train, case):
     name, f, tensors = _first_order_cases(train)[case]
     tensors = [t.requires_grad_() for t in tensors]
@@ -180,3 +181,23 @@ def test_lookups_of_any_shape(train, shape, dim):
     ids = torch.randint(0, 5, shape)
     train.lookup(t, ids).sum().backward()
     assert torch.equal(t.grad, torch.bincount(ids.reshape(-1), minlength=5)[:, None].expand(5, dim).float())
+
+
+def test_a_product_holds_neither_operand(train):
+    # what leads a second derivative back to them holds no memory of its own
+    x, w = torch.randn(3, 4).requires_grad_(), torch.randn(5, 4).requires_grad_()
+    y = train.product_fp8(2 * x, -w)
+    for link in y.grad_fn.links:
+        assert link.requires_grad and link.untyped_storage().nbytes() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_lists_of_either_type(train, dtype):
+    trainer, ids, logits = _trainer(train)
+    start, batch = trainer.table.clone(), torch.tensor([-1, 8, 5], dtype=torch.int32)
+    lists = torch.where(ids[:3] == batch.unsqueeze(1), -1, ids[:3])
+    want = trainer.step(batch, lists, logits[:3]), trainer.table.clone()
+    trainer.table.copy_(start)
+    got = trainer.step(batch.to(dtype), lists.to(dtype), logits[:3]), trainer.table
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
