@@ -833,8 +833,7 @@ int tessa_create(int device, tessa_ctx** out) {
   if (!ctx) return fail(TESSA_ERR_OOM, "context allocation failed");
   ctx->device = device;
   ctx->sm_count = prop.multiProcessorCount;
-  DeviceScope<CudaDevices> scope;
-  int r = scope.enter(device) == 0 ? TESSA_OK : fail(TESSA_ERR_CUDA, "device %d cannot be made current", device);
+  int r = bind(ctx);
   if (r == TESSA_OK) {
     if (cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking) != cudaSuccess) r = fail(TESSA_ERR_CUDA, "stream create failed");
   }

@@ -873,6 +873,15 @@ def _workspace(nbytes: int, device):
     return _torch.empty_strided((nbytes,), (1,), dtype=_torch.uint8, device=device) if nbytes else None
 
 
+def _context(dev: int) -> Context:
+    """context(dev); where that has to make one, the current device stays what it was."""
+    ctx = getattr(_tls, "ctx", {}).get(dev)
+    if ctx is None:
+        with _torch.cuda.device(_torch.cuda.current_device()):
+            ctx = context(dev)
+    return ctx
+
+
 def _written(out):
     """`out` holds other values now: a graph that saved it must find out, as after torch's own writes."""
     if not out.is_inference():
@@ -882,7 +891,7 @@ def _written(out):
 def async_status(ctx: Context | None = None, device: int = 0) -> None:
     """Waits for the current stream and raises what the calls of this section left (tessa_async_status)."""
     _lazy_torch()
-    ctx = ctx or context(device)
+    ctx = ctx or _context(device)
     C.check(C.load().tessa_async_status(ctx.handle, _stream(ctx.device)))
 
 
@@ -912,7 +921,7 @@ def embedding_lookup(table, ids, scale: float = 1.0, out=None, out_dtype=None, c
         res = out
     a = C.LookupArgs(table.data_ptr(), rows, stride, dim, code, flat.data_ptr(), id_bits, out_code, n, scale,
                      res.data_ptr(), out_stride)
-    C.check(C.load().tessa_embedding_lookup((ctx or context(dev)).handle, a, _stream(dev)))
+    C.check(C.load().tessa_embedding_lookup((ctx or _context(dev)).handle, a, _stream(dev)))
     if out is not None:
         _written(out)
     return res
@@ -957,7 +966,7 @@ def embedding_grad(dout, ids, table_rows: int, scale: float = 1.0, out_dtype=Non
     ws = _workspace(need.value, dout.device)
     a = C.LookupGradArgs(d2.data_ptr(), stride, dim, code, flat.data_ptr(), id_bits, out_code, n, scale,
                          1 if accumulate else 0, grad.data_ptr(), out_stride, table_rows)
-    C.check(lib.tessa_embedding_grad((ctx or context(dev)).handle, a, ws.data_ptr() if ws is not None else None,
+    C.check(lib.tessa_embedding_grad((ctx or _context(dev)).handle, a, ws.data_ptr() if ws is not None else None,
                                      need.value, _stream(dev)))
     if out is not None:
         _written(out)
@@ -983,7 +992,7 @@ def _quantize_fp8(x, along_rows: bool, along_cols: bool, ctx):
         ct, st = _empty(*cs, f8, device), _empty(*ss, u8, device)
     a = C.Fp8QuantizeArgs(x.data_ptr(), rows, cols, stride, code, 0, *((c.data_ptr(), s.data_ptr()) if along_rows else (None, None)),
                           *((ct.data_ptr(), st.data_ptr()) if along_cols else (None, None)))
-    C.check(C.load().tessa_quantize_fp8((ctx or context(dev)).handle, a, _stream(dev)))
+    C.check(C.load().tessa_quantize_fp8((ctx or _context(dev)).handle, a, _stream(dev)))
     return c, s, ct, st
 
 
@@ -1041,7 +1050,7 @@ def matmul_fp8(a_codes, a_scales, b_codes, b_scales, out_dtype=None, out=None, c
         _, _, out_stride, out_code = _matrix("out", out, dev)
         res = out
     lib = C.load()
-    handle = (ctx or context(dev)).handle
+    handle = (ctx or _context(dev)).handle
     need = ctypes.c_uint64()
     C.check(lib.tessa_matmul_fp8_workspace(handle, m, n, k, need))
     ws = _workspace(need.value, a_codes.device)
@@ -1088,7 +1097,7 @@ def _distill(logits, teacher_ids, teacher_logits, temperature, row_weights, want
     if want_grad:
         C.check(lib.tessa_distill_topk_workspace(a, need))
         ws = _workspace(need.value, device)
-    C.check(lib.tessa_distill_topk((ctx or context(dev)).handle, a, ws.data_ptr() if ws is not None else None,
+    C.check(lib.tessa_distill_topk((ctx or _context(dev)).handle, a, ws.data_ptr() if ws is not None else None,
                                    need.value, _stream(dev)))
     if out is not None:
         _written(out)

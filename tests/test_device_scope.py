@@ -64,10 +64,39 @@ def test_every_training_call_keeps_to_it():
         capi = f.read()
     assert "cudaSetDevice" not in train and "bind(" not in train
     assert train.count("TRY(async_begin(ctx, &c));") == 5
-    # the first call on a device also makes its context, and the last reference may go anywhere
-    for name in ("tessa::async_begin", "tessa_async_status", "tessa_create", "tessa_destroy"):
+    # the last reference to a context may go anywhere
+    for name in ("tessa::async_begin", "tessa_async_status", "tessa_destroy"):
         body = re.search(rf"(?:int|void) {name}\(.*?\n}}\n", capi, re.S).group(0)
         assert "scope" in body and "bind(" not in body and "cudaSetDevice" not in body, name
+
+
+def test_a_context_made_by_a_training_call(monkeypatch):
+    # in Python, as the C call that makes one leaves its device current
+    import contextlib
+    import threading
+
+    import torch
+    from shear_b200 import ops
+    current = [0]
+
+    @contextlib.contextmanager
+    def device(i):
+        before, current[0] = current[0], i
+        yield
+        current[0] = before
+
+    class Fake:
+        def __init__(self, dev):
+            current[0] = self.device = dev
+
+    ops._lazy_torch()
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(ops, "Context", Fake)
+    monkeypatch.setattr(ops, "_tls", threading.local())
+    made = ops._context(1)
+    assert made.device == 1 and current == [0]
+    assert ops._context(1) is made is ops.context(1) and ops._context(0) is not made and current == [0]
 
 
 @pytest.mark.gpu
@@ -78,9 +107,7 @@ def test_a_call_on_another_device():
         pytest.skip("needs two GPUs")
     table, ids = torch.randn(9, 8, device="cuda:1"), torch.arange(4, device="cuda:1")
     torch.cuda.set_device(0)
-    ctx = ops.Context(1)
-    got = ops.embedding_lookup(table, ids, ctx=ctx)
+    got = ops.embedding_lookup(table, ids)  # makes the thread's context
     assert torch.cuda.current_device() == 0
-    ops.async_status(ctx)
-    ctx.close()
+    ops.async_status(device=1)
     assert torch.cuda.current_device() == 0 and torch.equal(got, table[:4])
