@@ -12,9 +12,10 @@
 // that crosses a tile border leaves its part in the workspace, and a last kernel
 // adds each such run's parts.  Every tile holds as many entries however popular
 // one id is, so skew costs nothing but the parts.  131072 rows of 128 f32 into
-// 200000: 67 us, of which the sort 24 (latency; the rows that no id names are
-// cleared beside it), the tiles 17 (4 TB/s), parts 9; adding to the gradient
-// instead 51.
+// 200000, skewed ids: 65 us in a graph.  Under the profiler, whose cold launches
+// come to 82, the sort's four take 51 (39 without the clearing of other rows
+// beside it), the tiles 16 (4 TB/s), the parts 15; adding to the gradient
+// instead takes 49.
 #include "train_common.cuh"
 
 namespace tessa {
@@ -272,9 +273,9 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const SortAr
 // every pass in the same launch, an entry a thread.  Per pass each warp counts
 // its entries' digits, the CTAs read one another's totals, and every entry goes
 // to its place, in whichever CTA that is (the last pass: to global memory).  One
-// launch instead of two a pass, each nearly all latency: the gradient of 4096
-// entries takes 36 us instead of 44, of 16384 43 instead of 47; with more
-// entries a thread, 32768 take 52 instead of 46.
+// launch instead of two a pass, each nearly all latency: into 20000 rows of 128
+// f32 the gradient of 8192 entries takes 17 us instead of 22, of 16384 22
+// instead of 24.5.
 constexpr uint32_t kClusterChunk = 1024, kClusterWarps = kClusterChunk / 32;
 constexpr uint32_t kClusterMost = 16u * kClusterChunk;
 

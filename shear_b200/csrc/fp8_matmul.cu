@@ -22,11 +22,14 @@
 // of one row at a time, five instructions a column.)
 // Two accumulators: one is emptied while the next is summed.
 //
-// Measured (bf16 out): 8192 x 8192 x 8192 0.41 ms (2.7 PFLOP/s), 4096 x 200000 x
-// 768 0.62 ms (2.0 PFLOP/s and 2.6 TB/s of stores, where this GPU writes 3.9 TB/s
-// at most), 2048 x 16384 x 768 26 us, 2048 x 768 x 16384 30 us.  What bounds it
-// is one thread's rate of issuing MMAs, about 500 cycles a stage of four with
-// their scales, and the stores where K is short.
+// Measured (bf16 out): 8192 x 8192 x 8192 0.355 ms from a cool GPU (3.1 PFLOP/s),
+// 0.40 in a row, where the power cap sets the clock; the tensor pipe is active 89 %
+// of the cycles, which bounds it.  4096 x 200000 x 768 0.55 and 0.60 ms (2.7 TB/s
+// of stores, where a plain fill writes 7.3): the tensor pipe is active 61 %, a tile
+// takes 4700 cycles of which its six stages' MMAs are 2700.  The rest is the time
+// of a tile that does not grow with K (its start, its accumulator's way out through
+// two boxes a warp); which part of it counts has not been measured.  2048 x 16384 x
+// 768 26 us, 2048 x 768 x 16384 30 us.
 //
 // K may be split over units (few tiles, long K): each unit writes f32 parts to
 // the workspace and a second kernel adds them in order of K, so the result
